@@ -32,7 +32,11 @@ ext = CUDAExtension(
     libraries=["rccl"],
     extra_compile_args={
         "cxx": ["-O3"],
-        "nvcc": ["-O3", "--offload-arch=gfx950"],
+        # no packed fp32 instructions: some of their forms have given wrong
+        # results on these boards now and then
+        "nvcc": ["-O3", "--offload-arch=gfx950",
+                 "-Xclang", "-target-feature",
+                 "-Xclang", "-packed-fp32-ops"],
     },
 )
 
