@@ -38,7 +38,8 @@ def parse_args():
     p.add_argument("--peers-per-itr", type=int, default=1)
     p.add_argument(
         "--norm", type=str, default="fused",
-        help="batch-norm backend: miopen|native|fused",
+        help="batch-norm backend: miopen|native|fused, or layer (layer "
+             "norm over the channels)",
     )
     p.add_argument("--dtype", type=str, default="bf16", choices=["bf16", "fp32"])
     p.add_argument("--device", type=str, default="cuda")

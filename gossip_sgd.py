@@ -110,7 +110,9 @@ def build_parser():
                    help="samples per agent epoch in synthetic mode")
     p.add_argument("--model", default="resnet50", type=str)
     p.add_argument("--norm", default="fused", type=str,
-                   choices=["fused", "native", "miopen"])
+                   choices=["fused", "native", "miopen", "layer"],
+                   help="batch norm backend, or 'layer': layer norm over "
+                        "the channels, without per-rank statistics")
     p.add_argument("--conv_impl", default="miopen", type=str,
                    choices=["auto", "miopen", "gemm", "mfma"],
                    help="conv backend (auto: hand-written MFMA kernels on "

@@ -84,7 +84,7 @@ def build_parser():
     p.add_argument("--synthetic_size", default=2048, type=int)
     p.add_argument("--model", default="resnet50", type=str)
     p.add_argument("--norm", default="fused", type=str,
-                   choices=["fused", "native", "miopen"])
+                   choices=["fused", "native", "miopen", "layer"])
     p.add_argument("--num_classes", default=1000, type=int)
     p.add_argument("--device", default=None, choices=[None, "cuda", "cpu"])
     p.add_argument("--image_size", default=224, type=int)

@@ -28,6 +28,8 @@ ext = CUDAExtension(
         os.path.join(CSRC, "gemm1x1_kernels.hip"),
         os.path.join(CSRC, "conv3x3_kernels.hip"),
         os.path.join(CSRC, "bn_kernels.hip"),
+        os.path.join(CSRC, "layer_norm.cpp"),
+        os.path.join(CSRC, "layer_norm_kernels.hip"),
     ],
     libraries=["rccl"],
     extra_compile_args={

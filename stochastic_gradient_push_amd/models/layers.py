@@ -12,6 +12,10 @@ module provides:
   kernels (see ops/csrc/bn_kernels.hip) fusing
   normalize+scale+shift[+residual-add][+ReLU] in one pass and the
   backward reductions in two.
+* ``FusedLayerNorm`` / ``FusedLayerNorm2d`` — layer norm over the last
+  dimensions, or over the channels of each pixel, with the same fused
+  residual add and ReLU (see ops/norm.py).  No running statistics: nothing
+  that gossip, which mixes parameters only, leaves different on each rank.
 """
 
 import os
@@ -395,3 +399,73 @@ class FusedBatchNorm2d(nn.BatchNorm2d):
         if self.relu:
             y = torch.relu(y)
         return y
+
+
+class FusedLayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm``[+residual add][+ReLU] in hand-written CDNA4 kernels.
+
+    Keeps the input's dtype (also under autocast): bf16 or fp16 activations
+    with fp32 weights are read and written once.
+    """
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True,
+                 bias=True, relu=False):
+        super().__init__(normalized_shape, eps=eps,
+                         elementwise_affine=elementwise_affine, bias=bias)
+        self.relu = relu
+
+    def forward(self, x, residual=None):
+        from .. import ops as _o
+
+        dims = len(self.normalized_shape)
+        if tuple(x.shape[-dims:]) != self.normalized_shape:
+            raise ValueError(
+                f"FusedLayerNorm over {self.normalized_shape} got an input "
+                f"of shape {tuple(x.shape)}"
+            )
+        y = _o.layer_norm(
+            x.flatten(-dims),
+            None if self.weight is None else self.weight.flatten(),
+            None if self.bias is None else self.bias.flatten(),
+            eps=self.eps,
+            residual=None if residual is None else residual.flatten(-dims),
+            relu=self.relu,
+        )
+        return y.view(x.shape)
+
+
+class FusedLayerNorm2d(nn.Module):
+    """Layer norm over the channels of each pixel[+residual add][+ReLU] of
+    an NCHW tensor; the slot of :class:`FusedBatchNorm2d` in a network.
+
+    A channels_last input is read as it lies (a pixel's channels are one
+    contiguous row); others are copied first.  The output is
+    channels_last.
+    """
+
+    def __init__(self, num_channels, eps=1e-5, relu=False):
+        super().__init__()
+        self.num_channels = num_channels
+        self.eps = eps
+        self.relu = relu
+        self.weight = nn.Parameter(torch.ones(num_channels))
+        self.bias = nn.Parameter(torch.zeros(num_channels))
+
+    def extra_repr(self):
+        return f"{self.num_channels}, eps={self.eps}, relu={self.relu}"
+
+    def forward(self, x, residual=None):
+        from .. import ops as _o
+
+        if x.dim() != 4 or x.shape[1] != self.num_channels:
+            raise ValueError(
+                f"FusedLayerNorm2d({self.num_channels}) got an input of "
+                f"shape {tuple(x.shape)}"
+            )
+        y = _o.layer_norm(
+            x.permute(0, 2, 3, 1), self.weight, self.bias, eps=self.eps,
+            residual=None if residual is None
+            else residual.permute(0, 2, 3, 1),
+            relu=self.relu,
+        )
+        return y.permute(0, 3, 1, 2)

@@ -61,6 +61,14 @@ def conv1x1(cin: int, cout: int, stride: int = 1,
     return nn.Conv2d(cin, cout, 1, stride=stride, bias=False)
 
 
+def _fused_norm(fused):
+    """The norm with a fused residual add and ReLU that ``fused`` stands
+    for: a class, or True for the batch norm."""
+    from .layers import FusedBatchNorm2d
+
+    return FusedBatchNorm2d if fused is True else fused
+
+
 class BasicBlock(nn.Module):
     expansion = 1
 
@@ -74,11 +82,10 @@ class BasicBlock(nn.Module):
         self.downsample = downsample
         self.stride = stride
         if fused:
-            from .layers import FusedBatchNorm2d
-
-            self.bn1 = FusedBatchNorm2d(planes, relu=True)
+            norm = _fused_norm(fused)
+            self.bn1 = norm(planes, relu=True)
             # bn2 fuses the residual add + final relu
-            self.bn2 = FusedBatchNorm2d(planes, relu=True)
+            self.bn2 = norm(planes, relu=True)
         else:
             self.bn1 = norm_layer(planes)
             self.bn2 = norm_layer(planes)
@@ -113,12 +120,11 @@ class Bottleneck(nn.Module):
         self.downsample = downsample
         self.stride = stride
         if fused:
-            from .layers import FusedBatchNorm2d
-
-            self.bn1 = FusedBatchNorm2d(planes, relu=True)
-            self.bn2 = FusedBatchNorm2d(planes, relu=True)
+            norm = _fused_norm(fused)
+            self.bn1 = norm(planes, relu=True)
+            self.bn2 = norm(planes, relu=True)
             # bn3 fuses the residual add + final relu
-            self.bn3 = FusedBatchNorm2d(planes * self.expansion, relu=True)
+            self.bn3 = norm(planes * self.expansion, relu=True)
         else:
             self.bn1 = norm_layer(planes)
             self.bn2 = norm_layer(planes)
@@ -152,18 +158,17 @@ class ResNet(nn.Module):
         conv_impl: str = "miopen",
     ):
         super().__init__()
-        from .layers import FusedBatchNorm2d, make_norm
+        from .layers import FusedBatchNorm2d, FusedLayerNorm2d, make_norm
 
-        self._fused = norm == "fused"
+        # 'fused' and 'layer' take the residual and the ReLU into the norm
+        self._fused = {"fused": FusedBatchNorm2d,
+                       "layer": FusedLayerNorm2d}.get(norm, False)
         self._conv_impl = conv_impl
-        self._norm_layer = (
-            (lambda c: FusedBatchNorm2d(c, relu=False))
-            if self._fused else make_norm(norm)
-        )
+        self._norm_layer = self._fused or make_norm(norm)
         self.inplanes = 64
         self.conv1 = nn.Conv2d(3, 64, 7, stride=2, padding=3, bias=False)
         self.bn1 = (
-            FusedBatchNorm2d(64, relu=True) if self._fused
+            self._fused(64, relu=True) if self._fused
             else self._norm_layer(64)
         )
         self.relu = nn.ReLU(inplace=True)

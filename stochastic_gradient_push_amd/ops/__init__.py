@@ -316,3 +316,6 @@ def gather_multi_(ptr_table: torch.Tensor, offsets: torch.Tensor,
     """Gather scattered grad tensors (device pointer table) into the
     flat buffer in one launch (steal-mode grads)."""
     _ext_for(out).gather_multi_(ptr_table, offsets, out)
+
+
+from .norm import layer_norm  # noqa: E402,F401

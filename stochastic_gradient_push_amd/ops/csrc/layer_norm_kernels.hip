@@ -1,0 +1,578 @@
+// Layer norm over the last dimension (+residual)(+ReLU), forward and
+// backward, for gfx950 (CDNA4).  bf16, fp16 or fp32 rows, fp32 arithmetic.
+//
+//   mean = sum(x) / C            var = sum((x - mean)^2) / C
+//   hat  = (x - mean) * rstd     rstd = 1 / sqrt(var + eps)
+//   y    = relu(hat * w + b + res)
+//
+//   g    = dy where y > 0        dres = g
+//   dw   = sum_rows(g * hat)     db   = sum_rows(g)
+//   dx   = rstd * (g w - mean_cols(g w) - hat * mean_cols(g w hat))
+//
+// The variance comes from the centred values that are still in registers,
+// never from a difference of squares.
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace {
+
+template <typename T> struct Pack;
+template <> struct Pack<__bf16> {
+  static constexpr int N = 8;
+  typedef __bf16 V __attribute__((ext_vector_type(8)));
+};
+template <> struct Pack<_Float16> {
+  static constexpr int N = 8;
+  typedef _Float16 V __attribute__((ext_vector_type(8)));
+};
+template <> struct Pack<float> {
+  static constexpr int N = 4;
+  typedef float V __attribute__((ext_vector_type(4)));
+};
+
+// 16 bytes at any element: rows of an odd width start off a 16-byte border,
+// and global memory takes such an access in one instruction
+template <typename T>
+__device__ __forceinline__ typename Pack<T>::V ldv(const T* p) {
+  typedef typename Pack<T>::V U __attribute__((aligned(sizeof(T))));
+  return *reinterpret_cast<const U*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void stv(T* p, typename Pack<T>::V v) {
+  typedef typename Pack<T>::V U __attribute__((aligned(sizeof(T))));
+  *reinterpret_cast<U*>(p) = v;
+}
+
+// elements [c, c + N) of a row of C as floats, `fill` behind its end
+template <typename T>
+__device__ __forceinline__ void load(const T* row, int c, int C, float fill,
+                                     float* f) {
+  constexpr int N = Pack<T>::N;
+  if (c + N <= C) {
+    const typename Pack<T>::V v = ldv(row + c);
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = (float)v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = c + j < C ? (float)row[c + j] : fill;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store(T* row, int c, int C, const float* f) {
+  constexpr int N = Pack<T>::N;
+  if (c + N <= C) {
+    typename Pack<T>::V v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (T)f[j];
+    stv(row + c, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (c + j < C) row[c + j] = (T)f[j];
+  }
+}
+
+// a weight vector in the rows' type or in fp32; none at all: `none`
+template <typename T>
+__device__ __forceinline__ void load_w(const void* w, bool w32, int c, int C,
+                                       float none, float* f) {
+  constexpr int N = Pack<T>::N;
+  if (w == nullptr) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = none;
+  } else if (w32) {
+    const float* p = static_cast<const float*>(w);
+#pragma unroll
+    for (int j = 0; j < N; j += 4) load<float>(p, c + j, C, 0.f, f + j);
+  } else {
+    load<T>(static_cast<const T*>(w), c, C, 0.f, f);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void put_w(void* w, bool w32, int64_t c, float f) {
+  if (w32)
+    static_cast<float*>(w)[c] = f;
+  else
+    static_cast<T*>(w)[c] = (T)f;
+}
+
+// Sum of K values over the TPR threads of a row, the same in each of them.
+// Up to a wave: butterflies.  Above: a block has one row, its waves meet in
+// `lds` (K * TPR / 64 floats, not touched again before the next barrier).
+template <int TPR, int K>
+__device__ __forceinline__ void row_sum(float* v, float* lds) {
+#pragma unroll
+  for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o);
+  if (TPR > 64) {
+    constexpr int W = TPR / 64;
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) lds[k * W + wave] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[k] += lds[k * W + i];
+    }
+  }
+}
+
+constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// --------------------------------------------------------------- forward
+// TPR threads hold one row, VPT 16-byte vectors each.
+template <typename T, int TPR, int VPT>
+__global__ __launch_bounds__(block_of(TPR)) void k_ln_fwd(
+    const T* __restrict__ x, int64_t xs, const T* __restrict__ res,
+    int64_t rs, const void* __restrict__ w, const void* __restrict__ b,
+    bool w32, T* __restrict__ y, float* __restrict__ mean_out,
+    float* __restrict__ rstd_out, float eps, int64_t M, int C, bool relu) {
+  constexpr int N = Pack<T>::N;
+  constexpr int G = block_of(TPR) / TPR;
+  __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
+  const int t = threadIdx.x % TPR;
+  const int g = threadIdx.x / TPR;
+  float wv[VPT][N], bv[VPT][N];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    load_w<T>(w, w32, (t + i * TPR) * N, C, 1.f, wv[i]);
+    load_w<T>(b, w32, (t + i * TPR) * N, C, 0.f, bv[i]);
+  }
+  const float inv = 1.f / (float)C;
+  for (int64_t r = (int64_t)blockIdx.x * G + g; r < M;
+       r += (int64_t)gridDim.x * G) {
+    const T* xr = x + r * xs;
+    float f[VPT][N], s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      load<T>(xr, (t + i * TPR) * N, C, 0.f, f[i]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += f[i][j];
+    }
+    row_sum<TPR, 1>(&s, lds);
+    const float mean = s / (float)C;  // exact where the sum is
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        f[i][j] -= mean;
+        if ((t + i * TPR) * N + j < C) q += f[i][j] * f[i][j];
+      }
+    row_sum<TPR, 1>(&q, lds);
+    const float rstd = 1.f / sqrtf(q * inv + eps);
+    T* yr = y + r * C;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (t + i * TPR) * N;
+      float a[N];
+      if (res != nullptr) load<T>(res + r * rs, c, C, 0.f, a);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float z = f[i][j] * rstd * wv[i][j] + bv[i][j];
+        if (res != nullptr) z += a[j];
+        f[i][j] = relu && z <= 0.f ? 0.f : z;  // a NaN stays
+      }
+      store<T>(yr, c, C, f[i]);
+    }
+    if (mean_out != nullptr && t == 0) {
+      mean_out[r] = mean;
+      rstd_out[r] = rstd;
+    }
+  }
+}
+
+// Rows too long for registers: one block each, read three times.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_ln_fwd_long(
+    const T* __restrict__ x, int64_t xs, const T* __restrict__ res,
+    int64_t rs, const void* __restrict__ w, const void* __restrict__ b,
+    bool w32, T* __restrict__ y, float* __restrict__ mean_out,
+    float* __restrict__ rstd_out, float eps, int64_t M, int C, bool relu) {
+  constexpr int N = Pack<T>::N;
+  __shared__ float lds[16];
+  const float inv = 1.f / (float)C;
+  for (int64_t r = blockIdx.x; r < M; r += gridDim.x) {
+    const T* xr = x + r * xs;
+    float f[N], s = 0.f, q = 0.f;
+    for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
+      load<T>(xr, (int)c, C, 0.f, f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += f[j];
+    }
+    row_sum<1024, 1>(&s, lds);
+    const float mean = s / (float)C;  // exact where the sum is
+    for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
+      load<T>(xr, (int)c, C, mean, f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) q += (f[j] - mean) * (f[j] - mean);
+    }
+    row_sum<1024, 1>(&q, lds);
+    const float rstd = 1.f / sqrtf(q * inv + eps);
+    for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
+      float wv[N], bv[N], a[N];
+      load<T>(xr, (int)c, C, 0.f, f);
+      load_w<T>(w, w32, (int)c, C, 1.f, wv);
+      load_w<T>(b, w32, (int)c, C, 0.f, bv);
+      if (res != nullptr) load<T>(res + r * rs, (int)c, C, 0.f, a);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float z = (f[j] - mean) * rstd * wv[j] + bv[j];
+        if (res != nullptr) z += a[j];
+        f[j] = relu && z <= 0.f ? 0.f : z;
+      }
+      store<T>(y + r * C, (int)c, C, f);
+    }
+    if (mean_out != nullptr && threadIdx.x == 0) {
+      mean_out[r] = mean;
+      rstd_out[r] = rstd;
+    }
+  }
+}
+
+// -------------------------------------------------------------- backward
+// Same split.  Each thread keeps the sums of its columns over the rows of
+// its block: partials[block] = {dw[C], db[C]} in fp32, added up in a fixed
+// order by k_ln_bwd_sum.  With one block the sums are the gradients.
+template <typename T, int TPR, int VPT>
+__global__ __launch_bounds__(block_of(TPR)) void k_ln_bwd(
+    const T* __restrict__ dy, int64_t ds, const T* __restrict__ x,
+    int64_t xs, const T* __restrict__ y, const void* __restrict__ w,
+    bool w32, const float* __restrict__ mean, const float* __restrict__ rstd,
+    T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partials,
+    int64_t M, int C) {
+  constexpr int N = Pack<T>::N;
+  constexpr int BT = block_of(TPR);
+  constexpr int G = BT / TPR;
+  constexpr int W = BT / 64;
+  __shared__ float lds[TPR > 64 ? 2 * W : W * TPR * VPT * N];
+  const int t = threadIdx.x % TPR;
+  const int g = threadIdx.x / TPR;
+  float wv[VPT][N], sw[VPT][N], sb[VPT][N];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    load_w<T>(w, w32, (t + i * TPR) * N, C, 1.f, wv[i]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sw[i][j] = sb[i][j] = 0.f;
+  }
+  const float inv = 1.f / (float)C;
+  for (int64_t r = (int64_t)blockIdx.x * G + g; r < M;
+       r += (int64_t)gridDim.x * G) {
+    const float mu = mean[r], rs = rstd[r];
+    float h[VPT][N], gv[VPT][N], s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (t + i * TPR) * N;
+      load<T>(x + r * xs, c, C, mu, h[i]);  // hat = 0 behind the end
+      load<T>(dy + r * ds, c, C, 0.f, gv[i]);
+      if (y != nullptr) {
+        float a[N];
+        load<T>(y + r * C, c, C, 0.f, a);
+#pragma unroll
+        for (int j = 0; j < N; ++j) gv[i][j] = a[j] <= 0.f ? 0.f : gv[i][j];
+      }
+      if (dres != nullptr) store<T>(dres + r * C, c, C, gv[i]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        h[i][j] = (h[i][j] - mu) * rs;
+        sw[i][j] += gv[i][j] * h[i][j];
+        sb[i][j] += gv[i][j];
+        gv[i][j] *= wv[i][j];
+        s[0] += gv[i][j];
+        s[1] += gv[i][j] * h[i][j];
+      }
+    }
+    if (dx != nullptr) {
+      row_sum<TPR, 2>(s, lds);
+      const float m0 = s[0] * inv, m1 = s[1] * inv;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          gv[i][j] = rs * (gv[i][j] - m0 - h[i][j] * m1);
+        store<T>(dx + r * C, (t + i * TPR) * N, C, gv[i]);
+      }
+    }
+  }
+  if (partials == nullptr) return;
+  float* out = partials + (int64_t)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float v = half ? sb[i][j] : sw[i][j];
+        // the rows of a wave, then its block's waves
+#pragma unroll
+        for (int o = TPR; o < 64; o <<= 1) v += __shfl_xor(v, o);
+        const int c = (t + i * TPR) * N + j;
+        if (TPR > 64) {
+          if (c < C) out[half * C + c] = v;
+        } else if ((threadIdx.x & 63) < TPR) {
+          lds[(threadIdx.x >> 6) * TPR * VPT * N + c] = v;
+        }
+      }
+    if (TPR <= 64) {
+      __syncthreads();
+      for (int c = threadIdx.x; c < C; c += BT) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) v += lds[k * TPR * VPT * N + c];
+        out[half * C + c] = v;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Rows too long for registers: dx of one row by one block, and the columns'
+// sums by k_ln_bwd_cols.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_ln_bwd_long(
+    const T* __restrict__ dy, int64_t ds, const T* __restrict__ x,
+    int64_t xs, const T* __restrict__ y, const void* __restrict__ w,
+    bool w32, const float* __restrict__ mean, const float* __restrict__ rstd,
+    T* __restrict__ dx, T* __restrict__ dres, int64_t M, int C) {
+  constexpr int N = Pack<T>::N;
+  __shared__ float lds[32];
+  const float inv = 1.f / (float)C;
+  for (int64_t r = blockIdx.x; r < M; r += gridDim.x) {
+    const float mu = mean[r], rs = rstd[r];
+    float m0 = 0.f, m1 = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {
+      float s[2] = {0.f, 0.f};
+      for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
+        float h[N], gv[N], wv[N];
+        load<T>(x + r * xs, (int)c, C, mu, h);
+        load<T>(dy + r * ds, (int)c, C, 0.f, gv);
+        load_w<T>(w, w32, (int)c, C, 1.f, wv);
+        if (y != nullptr) {
+          float a[N];
+          load<T>(y + r * C, (int)c, C, 0.f, a);
+#pragma unroll
+          for (int j = 0; j < N; ++j) gv[j] = a[j] <= 0.f ? 0.f : gv[j];
+        }
+        if (pass == 0 && dres != nullptr)
+          store<T>(dres + r * C, (int)c, C, gv);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          h[j] = (h[j] - mu) * rs;
+          gv[j] *= wv[j];
+          s[0] += gv[j];
+          s[1] += gv[j] * h[j];
+          gv[j] = rs * (gv[j] - m0 - h[j] * m1);
+        }
+        if (pass == 1) store<T>(dx + r * C, (int)c, C, gv);
+      }
+      if (dx == nullptr) break;
+      if (pass == 0) {
+        row_sum<1024, 2>(s, lds);
+        m0 = s[0] * inv;
+        m1 = s[1] * inv;
+      }
+    }
+  }
+}
+
+// partials[by] of 256 * N columns over the rows by, by + gridDim.y, ...
+template <typename T>
+__global__ __launch_bounds__(256) void k_ln_bwd_cols(
+    const T* __restrict__ dy, int64_t ds, const T* __restrict__ x,
+    int64_t xs, const T* __restrict__ y, const float* __restrict__ mean,
+    const float* __restrict__ rstd, float* __restrict__ partials, int64_t M,
+    int C) {
+  constexpr int N = Pack<T>::N;
+  const int64_t c64 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
+  if (c64 >= C) return;
+  const int c = (int)c64;
+  float sw[N] = {0.f}, sb[N] = {0.f};
+  for (int64_t r = blockIdx.y; r < M; r += gridDim.y) {
+    const float mu = mean[r], rs = rstd[r];
+    float h[N], gv[N];
+    load<T>(x + r * xs, c, C, mu, h);
+    load<T>(dy + r * ds, c, C, 0.f, gv);
+    if (y != nullptr) {
+      float a[N];
+      load<T>(y + r * C, c, C, 0.f, a);
+#pragma unroll
+      for (int j = 0; j < N; ++j) gv[j] = a[j] <= 0.f ? 0.f : gv[j];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      sw[j] += gv[j] * ((h[j] - mu) * rs);
+      sb[j] += gv[j];
+    }
+  }
+  float* out = partials + (int64_t)blockIdx.y * 2 * C;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (c + j < C) {
+      out[c + j] = sw[j];
+      out[C + c + j] = sb[j];
+    }
+}
+
+// Column sums of partials [P][2C]: a block has 16 columns, 16 threads on
+// each, which add up in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ln_bwd_sum(
+    const float* __restrict__ partials, int P, int C, void* __restrict__ dw,
+    void* __restrict__ db, bool w32) {
+  __shared__ float lds[256];
+  const int cl = threadIdx.x & 15, k0 = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + cl;
+  float v = 0.f;
+  if (c < 2 * (int64_t)C)
+    for (int k = k0; k < P; k += 16) v += partials[(int64_t)k * 2 * C + c];
+  lds[threadIdx.x] = v;
+  __syncthreads();
+  if (k0 != 0 || c >= 2 * (int64_t)C) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) v += lds[k * 16 + cl];
+  if (c < C) {
+    if (dw != nullptr) put_w<T>(dw, w32, c, v);
+  } else if (db != nullptr) {
+    put_w<T>(db, w32, c - C, v);
+  }
+}
+
+// ---------------------------------------------------------------- launch
+// The narrowest row group that holds a row in registers: short rows share
+// a wave, rows of up to 256 vectors have one, longer ones a block.
+constexpr int MAX_VECTORS = 1024 * 4;
+
+#define LN_FOR_SHAPE(nv, CALL)                                     \
+  do {                                                             \
+    if ((nv) <= 8) { CALL(8, 1); }                                 \
+    else if ((nv) <= 16) { CALL(16, 1); }                          \
+    else if ((nv) <= 32) { CALL(32, 1); }                          \
+    else if ((nv) <= 64) { CALL(64, 1); }                          \
+    else if ((nv) <= 128) { CALL(64, 2); }                         \
+    else if ((nv) <= 256) { CALL(64, 4); }                         \
+    else if ((nv) <= 512) { CALL(256, 2); }                        \
+    else if ((nv) <= 1024) { CALL(256, 4); }                       \
+    else if ((nv) <= 2048) { CALL(512, 4); }                       \
+    else { CALL(1024, 4); }                                        \
+  } while (0)
+
+template <typename T>
+int vectors(int64_t C) {
+  return (int)((C + Pack<T>::N - 1) / Pack<T>::N);
+}
+
+int groups_of(int nv) {  // rows that a block of k_ln_fwd / k_ln_bwd has
+  return nv <= 8 ? 32 : nv <= 16 ? 16 : nv <= 32 ? 8 : nv <= 256 ? 4 : 1;
+}
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <typename T>
+void fwd(const void* x, int64_t xs, const void* res, int64_t rs,
+         const void* w, const void* b, bool w32, void* y, float* mean,
+         float* rstd, float eps, int64_t M, int C, bool relu,
+         hipStream_t s) {
+  const int nv = vectors<T>(C);
+  const T* xp = static_cast<const T*>(x);
+  const T* rp = static_cast<const T*>(res);
+  T* yp = static_cast<T*>(y);
+  if (nv > MAX_VECTORS) {
+    const int grid = (int)(M < 512 ? M : 512);
+    hipLaunchKernelGGL(k_ln_fwd_long<T>, dim3(grid), dim3(1024), 0, s, xp,
+                       xs, rp, rs, w, b, w32, yp, mean, rstd, eps, M, C,
+                       relu);
+    return;
+  }
+  int64_t grid = cdiv(M, groups_of(nv));
+  if (grid > 2048) grid = 2048;
+#define LN_FWD(TPR, VPT)                                              \
+  hipLaunchKernelGGL((k_ln_fwd<T, TPR, VPT>), dim3((unsigned)grid),   \
+                     dim3(block_of(TPR)), 0, s, xp, xs, rp, rs, w, b, \
+                     w32, yp, mean, rstd, eps, M, C, relu)
+  LN_FOR_SHAPE(nv, LN_FWD);
+#undef LN_FWD
+}
+
+template <typename T>
+int partial_rows(int64_t M, int C) {
+  const int nv = vectors<T>(C);
+  int64_t p = nv > MAX_VECTORS ? cdiv(M, 16) : cdiv(M, groups_of(nv));
+  return (int)(p < 512 ? p : 512);
+}
+
+template <typename T>
+void bwd(const void* dy, int64_t ds, const void* x, int64_t xs,
+         const void* y, const void* w, bool w32, const float* mean,
+         const float* rstd, void* dx, void* dres, float* partials, void* dw,
+         void* db, bool g32, int64_t M, int C, hipStream_t s) {
+  const int nv = vectors<T>(C);
+  const T* xp = static_cast<const T*>(x);
+  const T* dp = static_cast<const T*>(dy);
+  const T* yp = static_cast<const T*>(y);
+  T* dxp = static_cast<T*>(dx);
+  T* drp = static_cast<T*>(dres);
+  const int P = partial_rows<T>(M, C);
+  if (nv > MAX_VECTORS) {
+    if (dx != nullptr || dres != nullptr) {
+      const int grid = (int)(M < 512 ? M : 512);
+      hipLaunchKernelGGL(k_ln_bwd_long<T>, dim3(grid), dim3(1024), 0, s, dp,
+                         ds, xp, xs, yp, w, w32, mean, rstd, dxp, drp, M, C);
+    }
+    if (partials != nullptr) {
+      const dim3 grid((unsigned)cdiv(C, 256 * Pack<T>::N), (unsigned)P);
+      hipLaunchKernelGGL(k_ln_bwd_cols<T>, grid, dim3(256), 0, s, dp, ds, xp,
+                         xs, yp, mean, rstd, partials, M, C);
+    }
+  } else {
+#define LN_BWD(TPR, VPT)                                              \
+  hipLaunchKernelGGL((k_ln_bwd<T, TPR, VPT>), dim3(P),                \
+                     dim3(block_of(TPR)), 0, s, dp, ds, xp, xs, yp,   \
+                     w, w32, mean, rstd, dxp, drp, partials, M, C)
+    LN_FOR_SHAPE(nv, LN_BWD);
+#undef LN_BWD
+  }
+  if (partials != nullptr)
+    hipLaunchKernelGGL(k_ln_bwd_sum<T>,
+                       dim3((unsigned)cdiv(2 * (int64_t)C, 16)), dim3(256),
+                       0, s, partials, P, C, dw, db, g32);
+}
+
+}  // namespace
+
+// dtype: 0 fp32, 1 bf16, 2 fp16.  w32 / g32: weights (their gradients) are
+// fp32 rather than in the rows' type.  Any of res, w, b, mean, y, dx, dres,
+// partials, dw and db may be null.  M and C are positive.
+extern "C" {
+
+void sgp_layer_norm_fwd(int dtype, const void* x, int64_t xs,
+                        const void* res, int64_t rs, const void* w,
+                        const void* b, bool w32, void* y, float* mean,
+                        float* rstd, float eps, int64_t M, int C, bool relu,
+                        hipStream_t s) {
+  auto f = dtype == 0 ? fwd<float> : dtype == 1 ? fwd<__bf16> : fwd<_Float16>;
+  f(x, xs, res, rs, w, b, w32, y, mean, rstd, eps, M, C, relu, s);
+}
+
+int sgp_layer_norm_partials(int dtype, int64_t M, int C) {
+  return dtype == 0 ? partial_rows<float>(M, C) : partial_rows<__bf16>(M, C);
+}
+
+void sgp_layer_norm_bwd(int dtype, const void* dy, int64_t ds, const void* x,
+                        int64_t xs, const void* y, const void* w, bool w32,
+                        const float* mean, const float* rstd, void* dx,
+                        void* dres, float* partials, void* dw, void* db,
+                        bool g32, int64_t M, int C, hipStream_t s) {
+  auto f = dtype == 0 ? bwd<float> : dtype == 1 ? bwd<__bf16> : bwd<_Float16>;
+  f(dy, ds, x, xs, y, w, w32, mean, rstd, dx, dres, partials, dw, db, g32, M,
+    C, s);
+}
+
+}  // extern "C"
