@@ -32,6 +32,7 @@ from stochastic_gradient_push_amd import (
     UniformMixing,
 )
 from stochastic_gradient_push_amd.models import build_resnet
+from stochastic_gradient_push_amd.ops.fused_muon import FusedMuon
 from stochastic_gradient_push_amd.ops.fused_sgd import FusedSGD
 from stochastic_gradient_push_amd.utils import Meter, make_logger
 from stochastic_gradient_push_amd.utils.cluster_manager import ClusterManager
@@ -129,6 +130,13 @@ def build_parser():
     p.add_argument("--num_classes", default=1000, type=int)
     p.add_argument("--fused_sgd", default="True", type=str,
                    help="use the one-kernel flat-buffer SGD")
+    p.add_argument("--optimizer", default="sgd", type=str,
+                   choices=["sgd", "muon"],
+                   help="muon: orthogonalised momentum for every matrix, "
+                        "SGD for vectors (flat parameters only; --lr is "
+                        "then the lr of the orthogonalised updates)")
+    p.add_argument("--rest_lr", default=1.0, type=float,
+                   help="muon: lr of the vectors, as a multiple of --lr")
     p.add_argument("--device", default=None, choices=[None, "cuda", "cpu"])
     p.add_argument("--image_size", default=224, type=int)
     return p
@@ -195,6 +203,11 @@ def parse_args(argv=None):
 
     if args.all_reduce:
         assert args.graph_type == -1
+    if args.optimizer == "muon":
+        assert args.fused_sgd and not args.all_reduce, (
+            "--optimizer muon works on the gossip wrapper's flat parameters: "
+            "not with --all_reduce True or --fused_sgd False"
+        )
 
     if args.network_interface_type != "auto" and args.device == "cuda":
         try:
@@ -617,15 +630,20 @@ def main(argv=None):
                 ) else None
             ),
         )
-        if args.fused_sgd:
+        steal_grads = args.steal_grads == "on" or (
+            args.steal_grads == "auto" and args.device == "cuda"
+        )
+        if args.optimizer == "muon":
+            optimizer = FusedMuon(
+                model.flatp, lr=args.lr, momentum=args.momentum,
+                weight_decay=args.weight_decay, nesterov=args.nesterov,
+                rest_lr=args.rest_lr, steal_grads=steal_grads,
+            )
+        elif args.fused_sgd:
             optimizer = FusedSGD(
                 model.flatp, lr=args.lr, momentum=args.momentum,
                 weight_decay=args.weight_decay, nesterov=args.nesterov,
-                steal_grads=(
-                    args.steal_grads == "on"
-                    or (args.steal_grads == "auto"
-                        and args.device == "cuda")
-                ),
+                steal_grads=steal_grads,
             )
         else:
             optimizer = torch.optim.SGD(

@@ -30,6 +30,8 @@ ext = CUDAExtension(
         os.path.join(CSRC, "bn_kernels.hip"),
         os.path.join(CSRC, "layer_norm.cpp"),
         os.path.join(CSRC, "layer_norm_kernels.hip"),
+        os.path.join(CSRC, "muon.cpp"),
+        os.path.join(CSRC, "muon_kernels.hip"),
     ],
     libraries=["rccl"],
     extra_compile_args={

@@ -319,3 +319,4 @@ def gather_multi_(ptr_table: torch.Tensor, offsets: torch.Tensor,
 
 
 from .norm import layer_norm  # noqa: E402,F401
+from .muon import MuonPlan, muon_step_, newton_schulz  # noqa: E402,F401

@@ -691,10 +691,12 @@ void bn_bwd_apply_py(torch::Tensor x, torch::Tensor dy,
 
 void init_comm_core(py::module_& m);
 void init_layer_norm(py::module_& m);
+void init_muon(py::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   init_comm_core(m);
   init_layer_norm(m);
+  init_muon(m);
   m.doc() = "gfx950 fused gossip + batchnorm kernels";
   m.def("scale_", &scale_, "x *= a (in place, fused over flat buffer)");
   m.def("add_scale_", &add_scale_, "x = (x + r) * a");

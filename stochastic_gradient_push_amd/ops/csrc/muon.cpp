@@ -1,0 +1,278 @@
+// Newton-Schulz and Muon entry points: argument checks, outputs and
+// workspace for muon_kernels.hip.
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <torch/extension.h>
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
+#include <c10/hip/HIPStream.h>
+
+extern "C" {
+int sgp_ns_chunk();
+void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
+                       int batch, int tile, int steps, int split_steps,
+                       float a, float b, float c, float growth, float eps,
+                       void* work, double* partials, float* r,
+                       hipStream_t s);
+void sgp_muon_step(int dtype, float* p, const void* g, float* buf,
+                   void* shadow, const float* lr, float mu, float wd,
+                   float rest_lr, bool nesterov, int steps, float a, float b,
+                   float c, float growth, float eps, const void* tables,
+                   const int64_t* layout, void* work, double* partials,
+                   float* r, hipStream_t s);
+}
+
+namespace {
+
+// the kernels' records, as muon_kernels.hip has them
+struct Mat {
+  int64_t start, x_off, a_off;
+  int rows, cols, n, m, np, mp, chunk0, chunk1;
+  int e;
+  float scale;
+};
+struct Tile { int mat, tm, tn, pad; };
+struct Chunk { int64_t start; int count, mat; };
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A side is at most 2^15 (n m entries of 1 / sqrt(n m) times 2^e around 1,
+// e up to 13) and a matrix at most 2^30 values.
+void check_matrix(int64_t rows, int64_t cols) {
+  TORCH_CHECK(rows >= 1 && cols >= 1 && rows <= (1 << 20)
+              && cols <= (1 << 20) && rows * cols <= (int64_t(1) << 30)
+              && std::min(rows, cols) <= (1 << 15),
+              "newton_schulz: a matrix must have 1 to 2^20 rows and columns, "
+              "one of them at most 2^15, and at most 2^30 values, got ",
+              rows, " x ", cols);
+}
+
+Mat make_mat(int64_t start, int64_t rows, int64_t cols, int tile,
+             double scale) {
+  Mat q{};
+  q.start = start;
+  q.rows = (int)rows;
+  q.cols = (int)cols;
+  q.n = (int)std::min(rows, cols);
+  q.m = (int)std::max(rows, cols);
+  q.np = (int)(cdiv(q.n, tile) * tile);
+  q.mp = (int)(cdiv(q.m, tile) * tile);
+  q.chunk1 = (int)cdiv(rows * cols, sgp_ns_chunk());
+  q.e = std::min(13, std::ilogb(std::sqrt((double)rows * (double)cols)));
+  q.scale = (float)scale;
+  return q;
+}
+
+// fp16 values of workspace: X and its transpose twice, A and B, two planes
+int64_t work_size(int64_t x_total, int64_t a_total) {
+  return 8 * x_total + 4 * a_total;
+}
+
+int tile_for(int64_t n) { return n > 256 ? 128 : 64; }
+
+int dtype_code(const torch::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return 0;
+    case torch::kBFloat16: return 1;
+    case torch::kFloat16: return 2;
+    default:
+      TORCH_CHECK(false, what, " must be fp32, bf16 or fp16, got ",
+                  t.scalar_type());
+  }
+}
+
+hipStream_t stream_of(const torch::Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// g: [batch, rows, cols]
+torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
+                            int64_t split_steps, double a, double b,
+                            double c, double growth, double eps) {
+  TORCH_CHECK(g.is_cuda() && g.is_contiguous() && g.dim() == 3,
+              "newton_schulz: g must be a contiguous [batch, rows, cols] "
+              "device tensor");
+  const int dtype = dtype_code(g, "newton_schulz: g");
+  TORCH_CHECK(steps >= 1 && steps <= 100 && split_steps >= 0
+              && split_steps <= steps, "newton_schulz: steps out of range");
+  const c10::DeviceGuard guard(g.device());
+  torch::Tensor out = torch::empty_like(g);
+  if (g.numel() == 0) return out;
+  const int64_t batch = g.size(0);
+  check_matrix(g.size(1), g.size(2));
+  const int tile = tile_for(std::min(g.size(1), g.size(2)));
+  const Mat q = make_mat(0, g.size(1), g.size(2), tile, 1.0);
+  const int64_t x_total = batch * q.np * (int64_t)q.mp;
+  const int64_t a_total = batch * q.np * (int64_t)q.np;
+  TORCH_CHECK(x_total / 4096 < (int64_t(1) << 31)
+              && batch * q.chunk1 < (int64_t(1) << 31),
+              "newton_schulz: too many values in one call");
+  const auto opt = g.options();
+  torch::Tensor work = torch::empty({work_size(x_total, a_total)},
+                                    opt.dtype(torch::kFloat16));
+  torch::Tensor partials = torch::empty({batch * q.chunk1},
+                                        opt.dtype(torch::kFloat64));
+  torch::Tensor r = torch::empty({batch}, opt.dtype(torch::kFloat32));
+  sgp_newton_schulz(dtype, g.data_ptr(), out.data_ptr(), &q, (int)batch, tile,
+                    (int)steps, (int)split_steps, (float)a, (float)b,
+                    (float)c, (float)growth, (float)eps, work.data_ptr(),
+                    partials.data_ptr<double>(), r.data_ptr<float>(),
+                    stream_of(g));
+  C10_HIP_CHECK(hipGetLastError());
+  return out;
+}
+
+// The tables of a Muon step over a flat buffer of `total` values with
+// matrices (start, rows, cols, scale); everything between is the rest.
+// -> (uint8 tensor on the host, layout)
+std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
+    const std::vector<std::tuple<int64_t, int64_t, int64_t, double>>& mats,
+    int64_t total) {
+  int64_t widest = 1;
+  for (const auto& [start, rows, cols, scale] : mats) {
+    check_matrix(rows, cols);
+    widest = std::max(widest, std::min(rows, cols));
+  }
+  const int tile = tile_for(widest);
+  const int chunk = sgp_ns_chunk();
+  std::vector<Mat> m;
+  std::vector<Chunk> chunks;
+  std::vector<Tile> packs, syms, rects;
+  std::vector<std::pair<int64_t, int64_t>> taken;
+  int64_t x_total = 0, a_total = 0;
+  for (const auto& [start, rows, cols, scale] : mats) {
+    TORCH_CHECK(start >= 0 && start + rows * cols <= total,
+                "muon: a matrix lies outside the flat buffer");
+    Mat q = make_mat(start, rows, cols, tile, scale);
+    q.x_off = x_total;
+    q.a_off = a_total;
+    q.chunk0 = (int)chunks.size();
+    q.chunk1 += q.chunk0;
+    const int i = (int)m.size();
+    for (int64_t at = 0; at < rows * cols; at += chunk)
+      chunks.push_back({start + at,
+                        (int)std::min<int64_t>(chunk, rows * cols - at), i});
+    x_total += q.np * (int64_t)q.mp;
+    a_total += q.np * (int64_t)q.np;
+    for (int tm = 0; tm < q.np / 64; ++tm)
+      for (int tn = 0; tn < q.mp / 64; ++tn) packs.push_back({i, tm, tn, 0});
+    taken.push_back({start, start + rows * cols});
+    m.push_back(q);
+  }
+  // the longest sums first: what starts last should end soon
+  std::vector<int> order(m.size());
+  for (size_t i = 0; i < m.size(); ++i) order[i] = (int)i;
+  std::stable_sort(order.begin(), order.end(),
+                   [&](int x, int y) { return m[x].mp > m[y].mp; });
+  for (int i : order)
+    for (int tn = 0; tn < m[i].np / tile; ++tn)
+      for (int tm = 0; tm <= tn; ++tm) syms.push_back({i, tm, tn, 0});
+  std::stable_sort(order.begin(), order.end(),
+                   [&](int x, int y) { return m[x].np > m[y].np; });
+  for (int i : order)
+    for (int tm = 0; tm < m[i].np / tile; ++tm)
+      for (int tn = 0; tn < m[i].mp / tile; ++tn)
+        rects.push_back({i, tm, tn, 0});
+  std::sort(taken.begin(), taken.end());
+  int64_t at = 0;
+  auto rest = [&](int64_t to) {
+    for (; at < to; at += chunk)
+      chunks.push_back({at, (int)std::min<int64_t>(chunk, to - at), -1});
+  };
+  for (const auto& [from, to] : taken) {
+    TORCH_CHECK(from >= at, "muon: two matrices overlap");
+    rest(from);
+    at = to;
+  }
+  rest(total);
+  TORCH_CHECK(packs.size() < (size_t(1) << 31)
+              && chunks.size() < (size_t(1) << 31),
+              "muon: too many values in one plan");
+
+  const std::vector<int64_t> layout = {
+      (int64_t)m.size(), (int64_t)chunks.size(), (int64_t)packs.size(),
+      (int64_t)syms.size(), (int64_t)rects.size(), x_total, a_total, tile};
+  auto bytes = [](const auto& v) { return v.size() * sizeof(v[0]); };
+  torch::Tensor tables = torch::empty(
+      {(int64_t)(bytes(m) + bytes(chunks) + bytes(packs) + bytes(syms)
+                 + bytes(rects))},
+      torch::TensorOptions().dtype(torch::kUInt8));
+  uint8_t* to = tables.data_ptr<uint8_t>();
+  auto copy = [&](const auto& v) {
+    if (!v.empty()) std::memcpy(to, v.data(), bytes(v));
+    to += bytes(v);
+  };
+  copy(m);
+  copy(chunks);
+  copy(packs);
+  copy(syms);
+  copy(rects);
+  return {tables, layout};
+}
+
+void check_flat(const torch::Tensor& t, const char* name,
+                const torch::Tensor& p, torch::ScalarType dtype) {
+  TORCH_CHECK(t.is_cuda() && t.device() == p.device() && t.is_contiguous()
+              && t.dim() == 1 && t.numel() == p.numel()
+              && t.scalar_type() == dtype, "muon_step_: ", name,
+              " must be a contiguous ", dtype, " vector of ", p.numel(),
+              " values on the parameters' device");
+}
+
+void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
+                torch::optional<torch::Tensor> shadow,
+                const torch::Tensor& tables,
+                const std::vector<int64_t>& layout, int64_t total,
+                const torch::Tensor& lr, double momentum, double weight_decay,
+                double rest_lr, bool nesterov, int64_t steps, double a,
+                double b, double c, double growth, double eps) {
+  check_flat(p, "params", p, torch::kFloat32);
+  TORCH_CHECK(p.numel() == total, "muon_step_: the plan is for ", total,
+              " values, params has ", p.numel());
+  TORCH_CHECK(g.scalar_type() == torch::kFloat32
+              || g.scalar_type() == torch::kBFloat16,
+              "muon_step_: grads must be fp32 or bf16, got ",
+              g.scalar_type());
+  check_flat(g, "grads", p, g.scalar_type());
+  check_flat(buf, "momentum_buf", p, torch::kFloat32);
+  if (shadow.has_value())
+    check_flat(*shadow, "shadow", p, torch::kBFloat16);
+  TORCH_CHECK(lr.is_cuda() && lr.device() == p.device() && lr.numel() == 1
+              && lr.scalar_type() == torch::kFloat32,
+              "muon_step_: lr must be one fp32 value on the parameters' "
+              "device");
+  TORCH_CHECK(tables.device() == p.device(),
+              "muon_step_: the plan is for another device");
+  TORCH_CHECK(layout.size() == 8, "muon_step_: not a plan");
+  TORCH_CHECK(steps >= 1 && steps <= 100, "muon_step_: steps out of range");
+  const c10::DeviceGuard guard(p.device());
+  const auto opt = p.options();
+  torch::Tensor work = torch::empty({work_size(layout[5], layout[6])},
+                                    opt.dtype(torch::kFloat16));
+  torch::Tensor partials = torch::empty({std::max<int64_t>(1, layout[1])},
+                                        opt.dtype(torch::kFloat64));
+  torch::Tensor r = torch::empty({std::max<int64_t>(1, layout[0])}, opt);
+  sgp_muon_step(g.scalar_type() == torch::kFloat32 ? 0 : 1,
+                p.data_ptr<float>(), g.data_ptr(), buf.data_ptr<float>(),
+                shadow.has_value() ? shadow->data_ptr() : nullptr,
+                lr.data_ptr<float>(), (float)momentum, (float)weight_decay,
+                (float)rest_lr, nesterov, (int)steps, (float)a, (float)b,
+                (float)c, (float)growth, (float)eps, tables.data_ptr(),
+                layout.data(), work.data_ptr(), partials.data_ptr<double>(),
+                r.data_ptr<float>(), stream_of(p));
+  C10_HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace
+
+void init_muon(py::module_& m) {
+  m.def("newton_schulz", &newton_schulz,
+        "orthogonal factors of [batch, rows, cols] by Newton-Schulz steps");
+  m.def("muon_plan", &muon_plan,
+        "tables of a Muon step: (start, rows, cols, scale) of each matrix");
+  m.def("muon_step_", &muon_step_,
+        "momentum, Newton-Schulz and update over a flat buffer");
+}

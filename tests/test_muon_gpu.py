@@ -1,0 +1,422 @@
+"""Newton-Schulz and Muon kernels against the definition in 64 bits.
+
+Bounds are in the Frobenius norm.  X starts with norm 1; a rounding of size
+d relative to X, A or B in any step grows by at most a = 3.4445 in each step
+up to the result, so by a^5 = 485 in all.  A step rounds X, A and B to 22
+bits (2^-23) and accumulates three products in fp32; eight such roundings a
+step are allowed: 5 * 485 * 8 * 2^-23 = 2.3e-3 for a result whose norm is
+about sqrt(n), against 0.12 per rounding for values of 11 bits.  Sharper,
+where the input is noise: at most four times the error of the same formulas
+in fp32, two bits for 22-bit values instead of 24.
+"""
+
+import pytest
+import torch
+
+from stochastic_gradient_push_amd import GossipDataParallel, ops
+from stochastic_gradient_push_amd.models import resnet18
+from stochastic_gradient_push_amd.ops.flat import FlatParams
+from stochastic_gradient_push_amd.ops.fused_muon import FusedMuon
+
+from .test_muon_cpu import COEF, Net
+
+pytestmark = pytest.mark.gpu
+
+BOUND = 5 * 485 * 8 * 2.0 ** -23
+
+
+def dev():
+    return torch.device("cuda", 0)
+
+
+def factor(g, steps=5, coef=COEF, eps=1e-7):
+    """The definition, in 64 bits on the CPU."""
+    a, b, c = coef
+    x = g.detach().double().cpu()
+    x = x / (torch.linalg.vector_norm(x, dim=(-2, -1), keepdim=True) + eps)
+    for _ in range(steps):
+        s = x @ x.mT if x.shape[-2] <= x.shape[-1] else x.mT @ x
+        eye = torch.eye(s.shape[-1], dtype=s.dtype)
+        p = a * eye + s @ (b * eye + c * s)
+        x = p @ x if x.shape[-2] <= x.shape[-1] else x @ p
+    return x.to(g.device)
+
+
+def rounding(ref, dtype):
+    """Norm of one rounding to the type."""
+    return torch.finfo(dtype).eps / 2 * float(ref.norm())
+
+
+def strong(rows, cols, seed=0, batch=()):
+    """A few strong directions over noise."""
+    g = torch.Generator(device=dev()).manual_seed(seed)
+
+    def randn(*s):
+        return torch.randn(*s, generator=g, device=dev())
+
+    k = min(rows, cols, 3)
+    return randn(*batch, rows, cols) + torch.matmul(
+        randn(*batch, rows, k), randn(*batch, k, cols))
+
+
+# both tiles, their borders, both orientations
+SHAPES = [(1, 1), (1, 9), (7, 1), (3, 2), (16, 16), (63, 65), (64, 64),
+          (65, 64), (64, 576), (640, 40), (129, 257), (256, 256), (257, 300),
+          (300, 1000), (1000, 260), (512, 512), (385, 385)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+def test_shapes(shape, dtype):
+    g = strong(*shape, seed=sum(shape)).to(dtype)
+    out = ops.newton_schulz(g)
+    assert out.dtype == dtype and out.shape == g.shape
+    assert out.is_contiguous()
+    ref = factor(g)
+    # bf16: the last two steps round to 11 bits, which grows by a^2 = 12,
+    # in each of X, A and B
+    single = 6 * 12 * 2.0 ** -12 * float(ref.norm()) \
+        if dtype == torch.bfloat16 else 0.0
+    err = float((out.double() - ref).norm())
+    assert err <= BOUND + rounding(ref, dtype) + single, (
+        err, float(ref.norm()))
+
+
+@pytest.mark.parametrize("shape", [(64, 64), (200, 300), (128, 1152),
+                                   (512, 512), (700, 300)])
+def test_noise_against_fp32(shape):
+    g = torch.randn(*shape, device=dev())
+    ref = factor(g)
+    x = g.clone()
+    tall = shape[0] > shape[1]
+    x = x.T.contiguous() if tall else x
+    x = x / (x.norm() + 1e-7)
+    a, b, c = COEF
+    for _ in range(5):
+        s = x @ x.T
+        x = a * x + (b * s + c * (s @ s)) @ x
+    plain = float(((x.T if tall else x).double() - ref).norm())
+    err = float((ops.newton_schulz(g).double() - ref).norm())
+    assert err <= 4 * plain + 4 * 2.0 ** -24 * float(ref.norm()), (err, plain)
+    # bf16: no further off than twice its own rounding
+    g = g.bfloat16()
+    ref = factor(g)
+    err = float((ops.newton_schulz(g).double() - ref).norm())
+    own = float((ref.bfloat16().double() - ref).norm())
+    assert err <= 2 * own, (err, own)
+
+
+@pytest.mark.parametrize("batch,rows,cols", [
+    ((5,), 48, 80), ((2, 3), 100, 70), ((3,), 300, 270), ((17,), 16, 5)])
+def test_batches(batch, rows, cols):
+    g = strong(rows, cols, batch=batch)
+    out = ops.newton_schulz(g)
+    flat, each = g.view(-1, rows, cols), out.view(-1, rows, cols)
+    for i in range(flat.shape[0]):
+        # a matrix's result does not depend on what lies beside it
+        assert torch.equal(each[i], ops.newton_schulz(flat[i])), i
+
+
+def test_strides():
+    g = strong(70, 90, batch=(4,))
+    want = ops.newton_schulz(g)
+    wide = torch.randn(4, 71, 97, device=dev())
+    wide[:, 1:, 7:] = g
+    assert torch.equal(ops.newton_schulz(wide[:, 1:, 7:]), want)
+    assert torch.equal(ops.newton_schulz(g.mT.contiguous().mT), want)
+    assert torch.equal(ops.newton_schulz(g[::2]), want[::2])
+    same = ops.newton_schulz(g[:1].expand(3, 70, 90))
+    assert torch.equal(same, want[:1].expand(3, 70, 90))
+    # the transpose of the input gives the transpose of the result
+    assert torch.equal(ops.newton_schulz(g.mT), want.mT)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e-8, 1e-3, 1e15, 1e30])
+def test_scales(scale):
+    # far below eps the result is 485 g / eps, not 0; far above, squares
+    # leave fp32's range
+    g = strong(60, 100) * scale
+    ref = factor(g)
+    out = ops.newton_schulz(g)
+    r = float(g.double().norm() / (g.double().norm() + 1e-7))
+    assert float((out.double() - ref).norm()) <= BOUND * r + \
+        2.0 ** -149 * 100
+    assert float(out.double().norm()) >= 0.9 * float(ref.norm())
+
+
+def test_one_strong_entry():
+    # all of the norm in one value: the largest that X can hold
+    g = 1e-3 * torch.randn(512, 2048, device=dev())
+    g[100, 1000] = 1e6
+    for scale in (1.0, 1e-16):
+        ref = factor(g * scale)
+        out = ops.newton_schulz(g * scale)
+        assert bool(torch.isfinite(out).all())
+        assert float((out.double() - ref).norm()) <= BOUND
+
+
+def test_zeros_and_bad_values():
+    g = strong(70, 300, batch=(4,))
+    clean = ops.newton_schulz(g)
+    g[0] = 0
+    g[1, 3, 5] = float("nan")
+    g[2, 69, 299] = -float("inf")
+    out = ops.newton_schulz(g)
+    assert bool((out[0] == 0).all())
+    assert bool(torch.isnan(out[1:3]).all())
+    assert torch.equal(out[3], clean[3])
+    for eps in (0.0, 1e-7):
+        assert bool((ops.newton_schulz(torch.zeros_like(g[0]), eps=eps)
+                     == 0).all())
+
+
+@pytest.mark.parametrize("steps,coef", [
+    (1, COEF), (2, COEF), (10, COEF), (25, (1.5, -0.5, 0.0)),
+    (12, (1.875, -1.25, 0.375))])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_steps_and_coefficients(steps, coef, dtype):
+    g = torch.randn(90, 130, device=dev()).to(dtype)
+    ref = factor(g, steps, coef)
+    out = ops.newton_schulz(g, steps=steps, coefficients=coef)
+    # growth up to the result is at most that from the start to size 1: a
+    # singular value of noise starts above 1e-4 here
+    growth = min(coef[0] ** steps, 1e4)
+    bound = steps * growth * 8 * 2.0 ** -23
+    single = 6 * 16 * 2.0 ** -12 * float(ref.norm()) \
+        if dtype == torch.bfloat16 else 0.0
+    err = float((out.double() - ref).norm())
+    assert err <= bound + rounding(ref, dtype) + single
+
+
+def test_same_call_same_bits():
+    g = strong(300, 500, batch=(2,))
+    first = ops.newton_schulz(g)
+    assert all(torch.equal(ops.newton_schulz(g), first) for _ in range(3))
+
+
+def test_refusals():
+    g = torch.randn(4, 6, device=dev())
+    ext = ops._ext_for(g)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        ops.newton_schulz(g.clone().requires_grad_(True))
+    with torch.no_grad():
+        ops.newton_schulz(g.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ext.newton_schulz(g, 5, 5, *COEF, 4.0, 1e-7)
+    with pytest.raises(RuntimeError, match="2\\^20"):
+        ops.newton_schulz(torch.empty(1, (1 << 20) + 1, device=dev()))
+    plan = ops.MuonPlan([(0, 4, 6)], 24, "cuda")
+    flat = g.flatten().clone()
+    with pytest.raises(RuntimeError, match="momentum_buf"):
+        ops.muon_step_(flat, flat.clone(), flat.double(), plan, 0.1)
+    with pytest.raises(RuntimeError, match="grads"):
+        ops.muon_step_(flat, flat.half(), flat.clone(), plan, 0.1)
+    with pytest.raises(RuntimeError, match="shadow"):
+        ops.muon_step_(flat, flat.clone(), flat.clone(), plan, 0.1,
+                       shadow=flat.clone())
+    with pytest.raises(ValueError, match="plan is for"):
+        ops.muon_step_(flat, flat.clone(), flat.clone(),
+                       ops.MuonPlan([(0, 4, 6)], 24, "cpu"), 0.1)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ext.muon_plan([(0, 4, 6, 1.0), (5, 2, 2, 1.0)], 24)
+    with pytest.raises(RuntimeError, match="outside"):
+        ext.muon_plan([(4, 4, 6, 1.0)], 24)
+
+
+# ------------------------------------------------------------------- step
+
+def oracle(p, g, buf, matrices, lr, mu, wd, nesterov, rest_lr):
+    p, g, buf = p.double(), g.double(), buf.double()
+    inside = torch.zeros(p.numel(), dtype=torch.bool, device=p.device)
+    for start, rows, cols in matrices:
+        inside[start:start + rows * cols] = True
+    g = g + wd * p * ~inside
+    buf = mu * buf + g
+    u = g + mu * buf if nesterov else buf
+    new = torch.where(inside, p * (1 - lr * wd), p - lr * rest_lr * u)
+    for start, rows, cols in matrices:
+        part = slice(start, start + rows * cols)
+        scale = max(1.0, rows / cols) ** 0.5
+        new[part] -= lr * scale * factor(u[part].view(rows, cols)).reshape(-1)
+    return new, buf
+
+
+LAYOUTS = {
+    # odd places, gaps before, between and behind
+    "mixed": ([(5, 64, 147), (20000, 256, 64), (9500, 30, 300),
+               (40000, 1, 77), (40100, 77, 1), (50001, 300, 270)], 140007),
+    "one": ([(0, 40, 30)], 1200),
+    "none": ([], 20001),
+    "small": ([(i * 50, 5 + i % 3, 6) for i in range(40)], 2000),
+}
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nesterov", [False, True])
+def test_step(layout, dtype, nesterov):
+    matrices, total = LAYOUTS[layout]
+    torch.manual_seed(total)
+    plan = ops.MuonPlan(matrices, total, "cuda")
+    p, buf = (torch.randn(total, device=dev()) for _ in range(2))
+    g = torch.randn(total, device=dev()).to(dtype)
+    shadow = torch.empty(total, device=dev(), dtype=torch.bfloat16)
+    lr, mu, wd, rest_lr = 0.05, 0.9, 0.1, 0.3
+    for _ in range(2):
+        want, wbuf = oracle(p, g, buf, matrices, lr, mu, wd, nesterov,
+                            rest_lr)
+        ops.muon_step_(p, g, buf, plan, lr, momentum=mu, weight_decay=wd,
+                       nesterov=nesterov, rest_lr=rest_lr, shadow=shadow)
+        # a few roundings of values of at most about 10
+        assert float((buf.double() - wbuf).abs().max()) <= 64 * 2.0 ** -24
+        tol = 64 * 2.0 ** -24 * torch.ones_like(want)
+        for start, rows, cols in matrices:
+            tol[start:start + rows * cols] += \
+                lr * max(1.0, rows / cols) ** 0.5 * BOUND
+        assert bool(((p.double() - want).abs() <= tol).all())
+        for start, rows, cols in matrices:
+            part = slice(start, start + rows * cols)
+            scale = lr * max(1.0, rows / cols) ** 0.5
+            assert float((p[part].double() - want[part]).norm()) <= \
+                scale * BOUND + 8 * 2.0 ** -24 * float(want[part].norm())
+        assert torch.equal(shadow, p.bfloat16())
+
+
+def test_step_agrees_with_newton_schulz():
+    torch.manual_seed(0)
+    matrices = [(0, 100, 64), (6400, 64, 300)]
+    plan = ops.MuonPlan(matrices, 25600, "cuda")
+    g = torch.randn(25600, device=dev())
+    p, buf = torch.zeros_like(g), torch.zeros_like(g)
+    ops.muon_step_(p, g, buf, plan, 1.0, momentum=0.5, nesterov=False)
+    assert torch.equal(buf, g)
+    for start, rows, cols in matrices:
+        part = slice(start, start + rows * cols)
+        o = ops.newton_schulz(g[part].view(rows, cols)).reshape(-1)
+        scale = max(1.0, rows / cols) ** 0.5
+        assert float((p[part] + scale * o).abs().max()) <= 1e-6 * scale
+
+
+def test_optimizer_against_cpu():
+    torch.manual_seed(1)
+    cpu = Net()
+    gpu = Net()
+    gpu.load_state_dict(cpu.state_dict())
+    gpu.to(dev())
+    opts = []
+    for net in (cpu, gpu):
+        flatp = FlatParams(net, flatten_grads=True)
+        opts.append(FusedMuon(flatp, lr=0.1, weight_decay=0.01,
+                              sgd_params=[net.fc.weight], rest_lr=0.5))
+    for _ in range(3):
+        opts[0].flatp.flat_grad.normal_()
+        opts[1].flatp.flat_grad.copy_(opts[0].flatp.flat_grad)
+        for opt in opts:
+            opt.step()
+        # each within BOUND times lr of the definition, and so is the CPU
+        assert float((opts[0].flatp.flat - opts[1].flatp.flat.cpu())
+                     .abs().max()) <= 3 * 2 * 0.1 * BOUND
+
+
+def _training(steps, capture):
+    """A ResNet-18 with layer norm in the gossip wrapper: bf16 working
+    weights, stolen gradients, layer norm and Muon together."""
+    torch.manual_seed(7)
+    net = resnet18(num_classes=10, norm="layer").to(dev()).to(
+        memory_format=torch.channels_last)
+    gdp = GossipDataParallel(net, rank=0, world_size=1,
+                             working_dtype=torch.bfloat16)
+    opt = FusedMuon(gdp.flatp, lr=0.02, rest_lr=0.1, weight_decay=0.01,
+                    steal_grads=True)
+    x = torch.randn(4, 3, 64, 64, device=dev()).to(
+        memory_format=torch.channels_last)
+    y = torch.randint(0, 10, (4,), device=dev())
+
+    def step():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = torch.nn.functional.cross_entropy(net(x), y)
+        loss.backward()
+        opt.step()
+        opt.zero_grad()
+        return loss.detach()
+
+    if not capture:
+        for _ in range(steps):
+            loss = step()
+        return gdp, opt, loss
+    for _ in range(2):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    for _ in range(steps - 2):
+        graph.replay()
+        torch.cuda.synchronize()
+    return gdp, opt, loss
+
+
+def test_layer_norm_and_muon_train_together():
+    gdp, opt, loss = _training(3, capture=False)
+    assert bool(torch.isfinite(loss)) and bool(
+        torch.isfinite(gdp.flatp.flat).all())
+    flatp = gdp.flatp
+    assert torch.equal(flatp.shadow, flatp.flat[:flatp.n_cast].bfloat16())
+    # every matrix moved by a full-rank step: its norm says so
+    assert float(opt.momentum_buf.norm()) > 0
+    gdp.shutdown()
+
+
+def test_captured_training():
+    # (convolutions may sum in another order from run to run, so that whole
+    # trainings are not compared bit by bit; the step itself is, below)
+    gdp, _, loss = _training(5, capture=True)
+    assert bool(torch.isfinite(loss)) and bool(
+        torch.isfinite(gdp.flatp.flat).all())
+    gdp.shutdown()
+
+
+def test_captured_step():
+    matrices, total = LAYOUTS["mixed"]
+    torch.manual_seed(3)
+    plan = ops.MuonPlan(matrices, total, "cuda")
+    state = [torch.randn(total, device=dev()) for _ in range(3)]
+    lr = torch.tensor([0.05], device=dev())
+    eager = [t.clone() for t in state]
+    p, g, buf = state
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm up on copies
+        ops.muon_step_(p.clone(), g, buf.clone(), plan, lr)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.muon_step_(p, g, buf, plan, lr)
+        o = ops.newton_schulz(g[:1000 * 9].view(100, 90))
+    for k in range(4):
+        g.normal_()
+        eager[1].copy_(g)
+        lr.fill_(0.05 / (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.muon_step_(eager[0], eager[1], eager[2], plan, lr)
+        want = ops.newton_schulz(eager[1][:1000 * 9].view(100, 90))
+        for a, b in zip(state, eager):
+            assert torch.equal(a, b), k
+        assert torch.equal(o, want), k
+
+
+def test_two_streams_at_once():
+    g = [strong(200, 300, seed=i) for i in range(2)]
+    want = [ops.newton_schulz(t) for t in g]
+    streams = [torch.cuda.Stream() for _ in g]
+    torch.cuda.synchronize()
+    out = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                out[i].append(ops.newton_schulz(g[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in out[i])
