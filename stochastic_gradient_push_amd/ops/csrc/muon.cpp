@@ -12,9 +12,10 @@
 
 extern "C" {
 int sgp_ns_chunk();
+int64_t sgp_ns_big_tiles(int64_t tiles);
 void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
-                       int batch, int tile, int steps, int split_steps,
-                       float a, float b, float c, float growth, float eps,
+                       int batch, int steps, int split_steps, float a,
+                       float b, float c, float growth, float eps,
                        void* work, double* partials, float* r,
                        hipStream_t s);
 void sgp_muon_step(int dtype, float* p, const void* g, float* buf,
@@ -34,7 +35,7 @@ struct Mat {
   int e;
   float scale;
 };
-struct Tile { int mat, tm, tn, pad; };
+struct Tile { int mat, tm, tn, big; };
 struct Chunk { int64_t start; int count, mat; };
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -50,16 +51,15 @@ void check_matrix(int64_t rows, int64_t cols) {
               rows, " x ", cols);
 }
 
-Mat make_mat(int64_t start, int64_t rows, int64_t cols, int tile,
-             double scale) {
+Mat make_mat(int64_t start, int64_t rows, int64_t cols, double scale) {
   Mat q{};
   q.start = start;
   q.rows = (int)rows;
   q.cols = (int)cols;
   q.n = (int)std::min(rows, cols);
   q.m = (int)std::max(rows, cols);
-  q.np = (int)(cdiv(q.n, tile) * tile);
-  q.mp = (int)(cdiv(q.m, tile) * tile);
+  q.np = (int)(cdiv(q.n, 64) * 64);
+  q.mp = (int)(cdiv(q.m, 64) * 64);
   q.chunk1 = (int)cdiv(rows * cols, sgp_ns_chunk());
   q.e = std::min(13, std::ilogb(std::sqrt((double)rows * (double)cols)));
   q.scale = (float)scale;
@@ -70,8 +70,6 @@ Mat make_mat(int64_t start, int64_t rows, int64_t cols, int tile,
 int64_t work_size(int64_t x_total, int64_t a_total) {
   return 8 * x_total + 4 * a_total;
 }
-
-int tile_for(int64_t n) { return n > 256 ? 128 : 64; }
 
 int dtype_code(const torch::Tensor& t, const char* what) {
   switch (t.scalar_type()) {
@@ -103,8 +101,7 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
   if (g.numel() == 0) return out;
   const int64_t batch = g.size(0);
   check_matrix(g.size(1), g.size(2));
-  const int tile = tile_for(std::min(g.size(1), g.size(2)));
-  const Mat q = make_mat(0, g.size(1), g.size(2), tile, 1.0);
+  const Mat q = make_mat(0, g.size(1), g.size(2), 1.0);
   const int64_t x_total = batch * q.np * (int64_t)q.mp;
   const int64_t a_total = batch * q.np * (int64_t)q.np;
   TORCH_CHECK(x_total / 4096 < (int64_t(1) << 31)
@@ -116,7 +113,7 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
   torch::Tensor partials = torch::empty({batch * q.chunk1},
                                         opt.dtype(torch::kFloat64));
   torch::Tensor r = torch::empty({batch}, opt.dtype(torch::kFloat32));
-  sgp_newton_schulz(dtype, g.data_ptr(), out.data_ptr(), &q, (int)batch, tile,
+  sgp_newton_schulz(dtype, g.data_ptr(), out.data_ptr(), &q, (int)batch,
                     (int)steps, (int)split_steps, (float)a, (float)b,
                     (float)c, (float)growth, (float)eps, work.data_ptr(),
                     partials.data_ptr<double>(), r.data_ptr<float>(),
@@ -125,18 +122,45 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
   return out;
 }
 
+// The tiles of one product of all matrices: X X^T or A^2 (sym: on and above
+// the diagonal) or B X.  As many 128 x 128 tiles as fill the card, the
+// longest sums first, so that what starts last ends soon.
+std::vector<Tile> product_tiles(const std::vector<Mat>& m, bool sym) {
+  auto length = [&](const Tile& t) { return sym ? m[t.mat].mp : m[t.mat].np; };
+  std::vector<Tile> big, small;
+  for (int i = 0; i < (int)m.size(); ++i) {
+    const int nt = m[i].np / 64, mt = sym ? nt : m[i].mp / 64;
+    for (int tm = 0; tm < nt; ++tm)
+      for (int tn = sym ? tm : 0; tn < mt; ++tn)
+        if ((tm | 1) == nt || (tn | 1) == mt)
+          small.push_back({i, tm, tn, 0});
+        else if (!(tm & 1) && !(tn & 1))
+          big.push_back({i, tm, tn, 1});
+  }
+  auto longer = [&](const Tile& x, const Tile& y) {
+    return length(x) > length(y);
+  };
+  std::stable_sort(big.begin(), big.end(), longer);
+  const size_t keep = (size_t)sgp_ns_big_tiles((int64_t)big.size());
+  for (size_t i = keep; i < big.size(); ++i)
+    for (int k = 0; k < 4; ++k) {
+      const Tile t{big[i].mat, big[i].tm + (k >> 1), big[i].tn + (k & 1), 0};
+      if (!sym || t.tm <= t.tn) small.push_back(t);
+    }
+  big.resize(keep);
+  std::stable_sort(small.begin(), small.end(), longer);
+  big.insert(big.end(), small.begin(), small.end());
+  return big;
+}
+
 // The tables of a Muon step over a flat buffer of `total` values with
 // matrices (start, rows, cols, scale); everything between is the rest.
 // -> (uint8 tensor on the host, layout)
 std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
     const std::vector<std::tuple<int64_t, int64_t, int64_t, double>>& mats,
     int64_t total) {
-  int64_t widest = 1;
-  for (const auto& [start, rows, cols, scale] : mats) {
+  for (const auto& [start, rows, cols, scale] : mats)
     check_matrix(rows, cols);
-    widest = std::max(widest, std::min(rows, cols));
-  }
-  const int tile = tile_for(widest);
   const int chunk = sgp_ns_chunk();
   std::vector<Mat> m;
   std::vector<Chunk> chunks;
@@ -146,7 +170,7 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
   for (const auto& [start, rows, cols, scale] : mats) {
     TORCH_CHECK(start >= 0 && start + rows * cols <= total,
                 "muon: a matrix lies outside the flat buffer");
-    Mat q = make_mat(start, rows, cols, tile, scale);
+    Mat q = make_mat(start, rows, cols, scale);
     q.x_off = x_total;
     q.a_off = a_total;
     q.chunk0 = (int)chunks.size();
@@ -162,20 +186,8 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
     taken.push_back({start, start + rows * cols});
     m.push_back(q);
   }
-  // the longest sums first: what starts last should end soon
-  std::vector<int> order(m.size());
-  for (size_t i = 0; i < m.size(); ++i) order[i] = (int)i;
-  std::stable_sort(order.begin(), order.end(),
-                   [&](int x, int y) { return m[x].mp > m[y].mp; });
-  for (int i : order)
-    for (int tn = 0; tn < m[i].np / tile; ++tn)
-      for (int tm = 0; tm <= tn; ++tm) syms.push_back({i, tm, tn, 0});
-  std::stable_sort(order.begin(), order.end(),
-                   [&](int x, int y) { return m[x].np > m[y].np; });
-  for (int i : order)
-    for (int tm = 0; tm < m[i].np / tile; ++tm)
-      for (int tn = 0; tn < m[i].mp / tile; ++tn)
-        rects.push_back({i, tm, tn, 0});
+  syms = product_tiles(m, true);
+  rects = product_tiles(m, false);
   std::sort(taken.begin(), taken.end());
   int64_t at = 0;
   auto rest = [&](int64_t to) {
@@ -194,7 +206,7 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
 
   const std::vector<int64_t> layout = {
       (int64_t)m.size(), (int64_t)chunks.size(), (int64_t)packs.size(),
-      (int64_t)syms.size(), (int64_t)rects.size(), x_total, a_total, tile};
+      (int64_t)syms.size(), (int64_t)rects.size(), x_total, a_total};
   auto bytes = [](const auto& v) { return v.size() * sizeof(v[0]); };
   torch::Tensor tables = torch::empty(
       {(int64_t)(bytes(m) + bytes(chunks) + bytes(packs) + bytes(syms)
@@ -246,7 +258,7 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
               "device");
   TORCH_CHECK(tables.device() == p.device(),
               "muon_step_: the plan is for another device");
-  TORCH_CHECK(layout.size() == 8, "muon_step_: not a plan");
+  TORCH_CHECK(layout.size() == 7, "muon_step_: not a plan");
   TORCH_CHECK(steps >= 1 && steps <= 100, "muon_step_: steps out of range");
   const c10::DeviceGuard guard(p.device());
   const auto opt = p.options();

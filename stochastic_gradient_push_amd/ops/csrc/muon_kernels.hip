@@ -24,8 +24,13 @@
 // = r, which enters A as r^2 and the result as r, and 2^e follows what a
 // small r lets X grow to: a gradient far below eps loses no bits.
 //
-// n and m are padded with zeros to whole tiles, so the products have no
+// n and m are padded with zeros to multiples of 64, so the products have no
 // borders; zeros stay zeros in every step.
+//
+// Layout.  A plane of R rows holds 32 columns of all rows one after another,
+// then the next 32: what a tile loads of its rows for 32 of K is one
+// contiguous piece of memory, whole cache lines (rows along K would be used
+// in halves of lines).
 
 #include <hip/hip_runtime.h>
 
@@ -54,12 +59,24 @@ struct Mat {
 };
 static_assert(sizeof(Mat) == 64, "the host packs 64 bytes");
 
-struct Tile { int mat, tm, tn, pad; };
+// A tile of a product: rows from tm * 64, columns from tn * 64, 64 or 128
+// (big) of each.
+struct Tile { int mat, tm, tn, big; };
+
+// Blocks go to the 8 XCDs in turn, each of which has an L2 of its own: the
+// `n` numbers are dealt so that an XCD gets neighbours.
+__device__ __forceinline__ int by_xcd(int block, int n) {
+  const int xcd = block & 7, k = block >> 3, each = n >> 3, more = n & 7;
+  return xcd * each + (xcd < more ? xcd : more) + k;
+}
 
 // Equal matrices one after another: everything from the block's number.
+// The first n_big of a product's 128 x 128 tiles are worked on as such, the
+// others as four of 64 x 64, and what an odd number of 64s leaves over too.
 struct Uniform {
   Mat first;
   int batch;
+  int big_sym, big_rect;
   __device__ Mat mat(int i) const {
     Mat q = first;
     q.start += (int64_t)i * q.rows * q.cols;
@@ -70,31 +87,60 @@ struct Uniform {
     q.chunk1 = q.chunk0 + chunks;
     return q;
   }
-  // tile `id` of nt x mt tiles in each matrix
-  __device__ Tile grid_tile(int64_t id, int nt, int mt) const {
-    const int64_t per = (int64_t)nt * mt;
-    const int i = (int)(id / per), t = (int)(id % per);
-    return {i, t / mt, t % mt, 0};
-  }
-  // tile `id` of the nt (nt + 1) / 2 on and above the diagonal
-  __device__ Tile sym_tile(int64_t id, int nt) const {
-    const int64_t per = (int64_t)nt * (nt + 1) / 2;
-    const int i = (int)(id / per), t = (int)(id % per);
-    int tn = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+  // the pair tm <= tn with number t: 0 0, 0 1, 1 1, 0 2, ...
+  __device__ static void triangle(int t, int& tm, int& tn) {
+    tn = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
     while ((tn + 1) * (tn + 2) / 2 <= t) ++tn;
     while (tn * (tn + 1) / 2 > t) --tn;
-    return {i, t - tn * (tn + 1) / 2, tn, 0};
+    tm = t - tn * (tn + 1) / 2;
   }
-  __device__ Tile sym(int64_t id, int T) const {
-    return sym_tile(id, first.np / T);
+  __device__ Tile pair(int id, int per, int mb, bool sym) const {
+    Tile t;
+    t.mat = id / per;
+    const int k = id % per;
+    if (sym) {
+      triangle(k, t.tm, t.tn);
+    } else {
+      // down 4 rows before to the right: neighbours share both operands
+      const int nb = first.np / 128, top = k / (4 * mb) * 4;
+      const int rows = nb - top < 4 ? nb - top : 4, j = k - top * mb;
+      t.tm = top + j % rows;
+      t.tn = j / rows;
+    }
+    t.tm *= 2;
+    t.tn *= 2;
+    t.big = 1;
+    return t;
   }
-  __device__ Tile rect(int64_t id, int T) const {
-    return grid_tile(id, first.np / T, first.mp / T);
+  __device__ Tile tile(int id, bool sym, int n_big) const {
+    const int nt = first.np / 64, mt = sym ? nt : first.mp / 64;
+    const int nb = nt / 2, mb = mt / 2;
+    const int per = sym ? nb * (nb + 1) / 2 : nb * mb;
+    if (id < n_big) return pair(by_xcd(id, n_big), per, mb, sym);
+    const int fours = per * batch - n_big;
+    id = by_xcd(id - n_big, (int)gridDim.x - n_big);
+    if (id < 4 * fours) {
+      Tile t = pair(n_big + id / 4, per, mb, sym);
+      t.tm += (id >> 1) & 1;
+      t.tn += id & 1;
+      t.big = 0;
+      return t;
+    }
+    id -= 4 * fours;
+    // the last column of 64s, then the last row
+    const int down = mt & 1 ? nt : 0;
+    const int strip = down + (!sym && (nt & 1) ? 2 * mb : 0);
+    const int k = id % strip;
+    if (k < down) return {id / strip, k, mt - 1, 0};
+    return {id / strip, nt - 1, k - down, 0};
   }
-  __device__ Tile pack(int64_t id) const { return rect(id, 64); }
-  __device__ int chunk_mat(int64_t id) const {
-    return (int)(id / first.chunk1);
+  __device__ Tile sym(int id) const { return tile(id, true, big_sym); }
+  __device__ Tile rect(int id) const { return tile(id, false, big_rect); }
+  __device__ Tile pack(int id) const {
+    const int mt = first.mp / 64, per = first.np / 64 * mt, k = id % per;
+    return {id / per, k / mt, k % mt, 0};
   }
+  __device__ int chunk_mat(int id) const { return id / first.chunk1; }
 };
 
 // Matrices of any shapes: tables that the host has laid out.
@@ -104,9 +150,9 @@ struct Table {
   const Tile* rects;
   const Tile* packs;
   __device__ Mat mat(int i) const { return mats[i]; }
-  __device__ Tile sym(int64_t id, int) const { return syms[id]; }
-  __device__ Tile rect(int64_t id, int) const { return rects[id]; }
-  __device__ Tile pack(int64_t id) const { return packs[id]; }
+  __device__ Tile sym(int id) const { return syms[id]; }
+  __device__ Tile rect(int id) const { return rects[id]; }
+  __device__ Tile pack(int id) const { return packs[id]; }
 };
 
 // Sum over a block of 256 threads, the same in each; `lds` has 4 doubles.
@@ -202,10 +248,21 @@ struct Momentum {
 
 struct Planes { half_t *h, *l; };  // l may be null: hi alone
 
-__device__ __forceinline__ void put(const Planes& p, int64_t i, float v) {
-  const half_t h = hi_of(v);
-  p.h[i] = h;
-  if (p.l != nullptr) p.l[i] = lo_of(v, h);
+// Where a plane of `rows` rows has (row, col); 32 columns are together.
+__device__ __forceinline__ int64_t place(int row, int col, int rows) {
+  return (int64_t)(col >> 5) * rows * 32 + row * 32 + (col & 31);
+}
+
+__device__ __forceinline__ void put8(const Planes& p, int64_t i,
+                                     const float* v) {
+  half8 h, l;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    h[x] = hi_of(v[x]);
+    l[x] = lo_of(v[x], h[x]);
+  }
+  *reinterpret_cast<half8*>(p.h + i) = h;
+  if (p.l != nullptr) *reinterpret_cast<half8*>(p.l + i) = l;
 }
 
 // X and its transpose, 64 x 64 values a block; r[mat] = |G| / (|G| + eps).
@@ -237,12 +294,16 @@ __global__ __launch_bounds__(256) void k_ns_pack(
     tile[tall ? b : a][tall ? a : b] = v;
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < 4096; k += 256) {
-    const int a = k >> 6, b = k & 63;
-    put(x, q.x_off + (int64_t)(t.tm * 64 + a) * q.mp + t.tn * 64 + b,
-        tile[a][b]);
-    put(xt, q.x_off + (int64_t)(t.tn * 64 + a) * q.np + t.tm * 64 + b,
-        tile[b][a]);
+  for (int k = threadIdx.x; k < 512; k += 256) {
+    // 4 neighbours have the 32 values of a row that lie together
+    const int a = (k >> 2) & 63, b = (k >> 8) * 32 + (k & 3) * 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = tile[a][b + i];
+    put8(x, q.x_off + place(t.tm * 64 + a, t.tn * 64 + b, q.np), v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = tile[b + i][a];
+    put8(xt, q.x_off + place(t.tn * 64 + a, t.tm * 64 + b, q.mp), v);
   }
 }
 
@@ -260,6 +321,152 @@ __device__ __forceinline__ int x_exp(const Mat& q, float r, int step,
   const float grown = fminf((float)step * k.log2_growth, 1.f - log2f(r));
   const int shift = (int)ceilf(grown) - 2;
   return shift > 0 ? q.e - shift : q.e;
+}
+
+// Rows of 32 halves lie in LDS without padding, as the direct loads write
+// them.  Row r's four 16-byte pieces are stored in the order c ^ turn(r),
+// which spreads the 16 rows of a fragment over all banks.
+__device__ __forceinline__ int turn(int row) {
+  return ((row >> 1) & 3) ^ ((row >> 3) & 1);
+}
+
+__device__ __forceinline__ void load_lds(const half_t* from, half_t* to) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) void*)from,
+      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// The operands of a product: planes and first value of P's and Q's rows.
+struct Operands {
+  const half_t* at[4];  // P hi, Q hi, P lo, Q lo
+  int64_t next[2];      // from 32 of K to the next: of P, of Q
+  int K;
+};
+
+// acc += P Q^T over 32 of K: F x F fragments from rows p_row.. of the P
+// planes and q_row.. of the Q planes in LDS, one plane after another.
+template <bool SPLIT, int F>
+struct Fragments {
+  static constexpr int NP = SPLIT ? 2 : 1;
+  half8 a[NP][F], b[NP][F];
+  __device__ __forceinline__ void read(const half_t* lds, int plane,
+                                       int p_row, int q_row, int at) {
+#pragma unroll
+    for (int x = 0; x < NP; ++x)
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        a[x][i] = *reinterpret_cast<const half8*>(
+            lds + 2 * x * plane + (p_row + i * 16) * 32 + at);
+        b[x][i] = *reinterpret_cast<const half8*>(
+            lds + (2 * x + 1) * plane + (q_row + i * 16) * 32 + at);
+      }
+  }
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[F][F]) const {
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            a[0][i], b[0][j], acc[i][j], 0, 0, 0);
+        if (SPLIT) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              a[0][i], b[NP - 1][j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              a[NP - 1][i], b[0][j], acc[i][j], 0, 0, 0);
+        }
+      }
+  }
+};
+
+// Where lane l reads a fragment: row l % 16, 8 halves from 8 (l / 16).
+__device__ __forceinline__ int fragment_at(int lane) {
+  const int row = lane & 15;
+  return row * 32 + ((lane >> 4) ^ turn(row)) * 8;
+}
+// Where it loads: a direct load brings 16 rows, 4 lanes a row.
+__device__ __forceinline__ int load_at(int lane) {
+  const int row = lane >> 2;
+  return row * 32 + ((lane & 3) ^ turn(row)) * 8;
+}
+
+// One barrier: all direct loads have arrived and all reads are done.
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+constexpr int LDS_BYTES = 65536;  // two blocks on a CU; twice that: one
+
+// 128 x 128, a wave 64 x 64 of it.  Two buffers: while one is multiplied,
+// the next 32 of K are on their way into the other.
+template <bool SPLIT>
+__device__ __forceinline__ void product128(const Operands& o, half_t* lds,
+                                           f32x4 (&acc)[4][4]) {
+  constexpr int NP = SPLIT ? 2 : 1, PLANE = 128 * 32;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int from = load_at(lane);
+  auto fetch = [&](int kt, half_t* to) {
+#pragma unroll
+    for (int x = 0; x < 2 * NP; ++x)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        load_lds(o.at[x] + kt * o.next[x & 1] + (i * 4 + wave) * 512 + from,
+                 to + x * PLANE + (i * 4 + wave) * 512);
+  };
+  const int at = fragment_at(lane);
+  const int KT = o.K / 32;
+  fetch(0, lds);
+  for (int kt = 0; kt < KT; ++kt) {
+    half_t* now = lds + (kt & 1) * 2 * NP * PLANE;
+    arrive();
+    if (kt + 1 < KT) fetch(kt + 1, lds + (~kt & 1) * 2 * NP * PLANE);
+    Fragments<SPLIT, 4> f;
+    f.read(now, PLANE, (wave >> 1) * 64, (wave & 1) * 64, at);
+    f.multiply(acc);
+  }
+}
+
+// 64 x 64, the whole of it by each wave over a quarter of K: 16 fragments
+// from 8 loads, as in the large tile, and no barrier.  A wave's loads go to
+// its own part of LDS; once its fragments are in registers the next are on
+// their way while it multiplies.  `deep`: the block has twice the LDS, and
+// a wave loads two steps ahead.
+template <bool SPLIT>
+__device__ __forceinline__ void product64(const Operands& o, half_t* lds,
+                                          bool deep, f32x4 (&acc)[4][4]) {
+  constexpr int NP = SPLIT ? 2 : 1, PLANE = 64 * 32, L = 8 * NP;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  half_t* own = lds + wave * (LDS_BYTES / 8);
+  const int from = load_at(lane);
+  auto fetch = [&](int kt, half_t* to) {
+#pragma unroll
+    for (int x = 0; x < 2 * NP; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        load_lds(o.at[x] + kt * o.next[x & 1] + i * 512 + from,
+                 to + x * PLANE + i * 512);
+  };
+  const int at = fragment_at(lane);
+  const int KT = o.K / 32, ahead = deep ? 8 : 4;
+  half_t* now = own;
+  half_t* next = deep ? own + LDS_BYTES / 2 : own;
+  if (wave < KT) fetch(wave, now);
+  if (deep && wave + 4 < KT) fetch(wave + 4, next);
+  for (int kt = wave; kt < KT; kt += 4) {
+    if (deep && kt + 4 < KT)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    Fragments<SPLIT, 4> f;
+    f.read(now, PLANE, 0, 0, at);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (kt + ahead < KT) fetch(kt + ahead, now);
+    f.multiply(acc);
+    half_t* t = now;
+    now = next;
+    next = t;
+  }
 }
 
 // Where the last product goes: a tensor, or the parameters.
@@ -284,117 +491,157 @@ struct ToParams {
 };
 struct ToPlanes {};  // not the last product
 
-// C = P Q^T, one T x T tile a block, 4 waves of T/2 x T/2, K in steps of 32.
-template <int T, bool SPLIT, int MODE, class Src, class Out>
-__global__ __launch_bounds__(256) void k_ns_gemm(
+// C = P Q^T for one tile, and what its product makes of it:
+//   GRAM   A = X X^T            stored at its place and mirrored
+//   POLY   B = a I + b A + c A^2     likewise
+//   APPLY  X = B X              stored, and transposed beside it; the last
+//                               one goes to `out`
+// Rounding, scaling and stores go through a 64-row image of the sums in LDS,
+// from which 8 lanes read 64 neighbours of a row, or of a column: a stride
+// of an odd number of words keeps both free of conflicts.
+template <bool SPLIT, int MODE, class Src, class Out>
+__global__ __launch_bounds__(256, 2) void k_ns_gemm(
     Src src, Planes P, Planes Q, Planes C, Planes D, Out out,
-    const float* __restrict__ r, Coef k, int step) {
-  constexpr int F = T / 32;            // 16 x 16 fragments a wave, a side
-  constexpr int S = 40;                // a row in LDS: 32 + 8 of padding
-  constexpr int V = T * 4 / 256;       // 16-byte pieces a thread, a plane
-  constexpr int NP = SPLIT ? 2 : 1;    // planes
-  __shared__ half_t lp[NP][T * S], lq[NP][T * S];
-  const Tile t = MODE == APPLY ? src.rect(blockIdx.x, T)
-                               : src.sym(blockIdx.x, T);
+    const float* __restrict__ r, Coef k, int step, bool deep) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  half_t* lds = reinterpret_cast<half_t*>(lds_raw);
+  float* image = reinterpret_cast<float*>(lds_raw);
+  constexpr bool LAST = MODE == APPLY && !__is_same(Out, ToPlanes);
+  const Tile t = MODE == APPLY ? src.rect(blockIdx.x) : src.sym(blockIdx.x);
+  if (MODE != APPLY && t.tm > t.tn) return;  // below the diagonal
   const Mat q = src.mat(t.mat);
   const int K = MODE == GRAM ? q.mp : q.np;
-  const int64_t p_off = (MODE == GRAM ? q.x_off : q.a_off)
-                        + (int64_t)t.tm * T * K;
-  const int64_t q_off = (MODE == POLY ? q.a_off : q.x_off)
-                        + (int64_t)t.tn * T * K;
+  const int q_rows = MODE == APPLY ? q.mp : q.np;
+  const int64_t p_off = (MODE == GRAM ? q.x_off : q.a_off) + t.tm * 64 * 32;
+  const int64_t q_off = (MODE == POLY ? q.a_off : q.x_off) + t.tn * 64 * 32;
+  const Operands o{{P.h + p_off, Q.h + q_off, SPLIT ? P.l + p_off : nullptr,
+                    SPLIT ? Q.l + q_off : nullptr},
+                   {(int64_t)q.np * 32, (int64_t)q_rows * 32}, K};
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = (wave >> 1) * (T / 2), wn = (wave & 1) * (T / 2);
 
-  f32x4 acc[F][F];
+  f32x4 acc[4][4];
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < F; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (t.big)
+    product128<SPLIT>(o, lds, acc);
+  else
+    product64<SPLIT>(o, lds, deep, acc);
 
-  for (int k0 = 0; k0 < K; k0 += 32) {
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int piece = threadIdx.x + v * 256;
-      const int row = piece >> 2, c = (piece & 3) * 8;
-      const int64_t from = (int64_t)row * K + k0 + c;
-      *reinterpret_cast<half8*>(&lp[0][row * S + c]) =
-          *reinterpret_cast<const half8*>(P.h + p_off + from);
-      *reinterpret_cast<half8*>(&lq[0][row * S + c]) =
-          *reinterpret_cast<const half8*>(Q.h + q_off + from);
-      if (SPLIT) {
-        *reinterpret_cast<half8*>(&lp[NP - 1][row * S + c]) =
-            *reinterpret_cast<const half8*>(P.l + p_off + from);
-        *reinterpret_cast<half8*>(&lq[NP - 1][row * S + c]) =
-            *reinterpret_cast<const half8*>(Q.l + q_off + from);
-      }
-    }
-    __syncthreads();
-    half8 a[NP][F], b[NP][F];
-#pragma unroll
-    for (int x = 0; x < NP; ++x)
-#pragma unroll
-      for (int i = 0; i < F; ++i) {
-        const int at = (i * 16 + (lane & 15)) * S + (lane >> 4) * 8;
-        a[x][i] = *reinterpret_cast<const half8*>(&lp[x][wm * S + at]);
-        b[x][i] = *reinterpret_cast<const half8*>(&lq[x][wn * S + at]);
-      }
-#pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-      for (int j = 0; j < F; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            a[0][i], b[0][j], acc[i][j], 0, 0, 0);
-        if (SPLIT) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              a[0][i], b[NP - 1][j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              a[NP - 1][i], b[0][j], acc[i][j], 0, 0, 0);
-        }
-      }
-  }
-
-  const float rr = MODE == POLY ? 0.f : r[t.mat];
-  const int e = MODE == POLY ? 0 : x_exp(q, rr, step, k);
   // what the sums are multiplied with: powers of two, and r or its square
   float f = 1.f / A_SCALE;
-  if (MODE == GRAM) f = ldexpf(rr * rr, -2 * e) * A_SCALE;
-  if (MODE == APPLY) {
-    if constexpr (__is_same(Out, ToPlanes))
-      f = ldexpf(1.f / B_SCALE, x_exp(q, rr, step + 1, k) - e);
-    else
+  if (MODE != POLY) {
+    const float rr = r[t.mat];
+    const int e = x_exp(q, rr, step, k);
+    if (MODE == GRAM)
+      f = ldexpf(rr * rr, -2 * e) * A_SCALE;
+    else if (LAST)
       f = ldexpf(rr / B_SCALE, -e);
+    else
+      f = ldexpf(1.f / B_SCALE, x_exp(q, rr, step + 1, k) - e);
   }
+
+  if (!t.big) {
+    // the sums of all four waves: each gets a quarter of the rows
+    f32x4* all = reinterpret_cast<f32x4*>(lds_raw);
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < F; ++j)
+      for (int j = 0; j < 4; ++j)
+        all[((wave * 4 + i) * 4 + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int row = t.tm * T + wm + i * 16 + (lane >> 4) * 4 + x;
-        const int col = t.tn * T + wn + j * 16 + (lane & 15);
-        float v = acc[i][j][x] * f;
-        if (MODE == APPLY) {
-          if constexpr (__is_same(Out, ToPlanes)) {
-            put(C, q.x_off + (int64_t)row * q.mp + col, v);
-            put(D, q.x_off + (int64_t)col * q.np + row, v);
-          } else if (row < q.n && col < q.m) {
-            const int64_t at = q.rows > q.cols
-                ? (int64_t)col * q.cols + row : (int64_t)row * q.cols + col;
-            out.put(q.start + at, v, q);
-          }
+    for (int j = 0; j < 4; ++j) {
+      f32x4 v = all[(wave * 4 + j) * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < 4; ++w)
+        v += all[((w * 4 + wave) * 4 + j) * 64 + lane];
+      acc[0][j] = v;
+    }
+  }
+
+  const int W = t.big ? 128 : 64, S = W + 1;
+  const int row0 = t.tm * 64, col0 = t.tn * 64;
+  for (int part = 0; part < W / 64; ++part) {
+    // a big tile: the upper, then the lower two waves' sums; a small one:
+    // every wave's quarter
+    __syncthreads();
+    if (!t.big || (wave >> 1) == part) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t.big || i == 0)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              image[((t.big ? i : wave) * 16 + (lane >> 4) * 4 + x) * S
+                    + (t.big ? (wave & 1) * 64 : 0) + j * 16 + (lane & 15)] =
+                  acc[i][j][x];
+    }
+    __syncthreads();
+    const int rp = row0 + part * 64;  // the image's first row
+    const bool mirror = MODE == APPLY ? !LAST : t.tm != t.tn;
+    const bool tall = LAST && q.rows > q.cols;
+    // along rows: 4 neighbours have 32 columns, the next 4 the next row
+    if (!tall) {
+      for (int u = threadIdx.x; u < 8 * W; u += 256) {
+        const int row = (u >> 2) & 63, col = (u >> 8) * 32 + (u & 3) * 8;
+        float v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = image[row * S + col + x] * f;
+        if constexpr (LAST) {
+          const int64_t at = q.start + (int64_t)(rp + row) * q.cols;
+          if (rp + row < q.n)
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              if (col0 + col + x < q.m)
+                out.put(at + col0 + col + x, v[x], q);
+        } else if constexpr (MODE == APPLY) {
+          put8(C, q.x_off + place(rp + row, col0 + col, q.np), v);
         } else {
+          const int64_t at = q.a_off + place(rp + row, col0 + col, q.np);
           if (MODE == POLY) {
-            const int64_t at = q.a_off + (int64_t)row * q.np + col;
-            float av = (float)P.h[at];
-            if (SPLIT) av += (float)P.l[at];
-            v = (k.b * av + k.c * v) * (B_SCALE / A_SCALE)
-                + (row == col ? k.a * B_SCALE : 0.f);
+            const half8 h = *reinterpret_cast<const half8*>(P.h + at);
+            half8 l = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (SPLIT) l = *reinterpret_cast<const half8*>(P.l + at);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              v[x] = (k.b * ((float)h[x] + (float)l[x]) + k.c * v[x])
+                     * (B_SCALE / A_SCALE);
+              if (rp + row == col0 + col + x) v[x] += k.a * B_SCALE;
+              if (mirror) image[row * S + col + x] = v[x];
+            }
           }
-          put(C, q.a_off + (int64_t)row * q.np + col, v);
-          if (t.tm != t.tn) put(C, q.a_off + (int64_t)col * q.np + row, v);
+          put8(C, at, v);
         }
       }
+    }
+    // along columns likewise: their transposed places
+    if (mirror || tall) {
+      if (MODE == POLY) __syncthreads();
+      for (int u = threadIdx.x; u < 8 * W; u += 256) {
+        const int col = (u >> 2) & (W - 1);
+        const int row = (u >> (t.big ? 9 : 8)) * 32 + (u & 3) * 8;
+        float v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          v[x] = image[(row + x) * S + col] * (MODE == POLY ? 1.f : f);
+        if constexpr (LAST) {
+          const int64_t at = q.start + (int64_t)(col0 + col) * q.cols;
+          if (col0 + col < q.m)
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              if (rp + row + x < q.n) out.put(at + rp + row + x, v[x], q);
+        } else if constexpr (MODE == APPLY) {
+          put8(D, q.x_off + place(col0 + col, rp + row, q.mp), v);
+        } else {
+          put8(C, q.a_off + place(col0 + col, rp + row, q.np), v);
+        }
+      }
+    }
+  }
 }
 
 // Workspace, in fp16 values: X and its transpose twice, A and B, each as
@@ -422,61 +669,78 @@ Work split_work(void* base, int64_t x_total, int64_t a_total) {
 
 Planes planes(Planes p, bool lo) { return {p.h, lo ? p.l : nullptr}; }
 
-template <int T, bool SPLIT, class Src, class Out>
+template <bool SPLIT, class Src, class Out>
 void ns_step(Src src, const Work& w, int step, bool next_split, bool last,
-             Out out, const float* r, Coef k, int64_t n_sym, int64_t n_rect,
+             Out out, const float* r, Coef k, int n_sym, int n_rect,
              hipStream_t s) {
   const int now = step & 1;
-  const dim3 block(256), sym((unsigned)n_sym), rect((unsigned)n_rect);
+  const dim3 block(256), sym(n_sym), rect(n_rect);
+  // a block for every CU at most: it has the CU's LDS for itself
+  const bool deep_sym = n_sym <= 256, deep_rect = n_rect <= 256;
+  const int lds_sym = deep_sym ? 2 * LDS_BYTES : LDS_BYTES;
+  const int lds_rect = deep_rect ? 2 * LDS_BYTES : LDS_BYTES;
   const Planes x = w.x[now], xt = w.xt[now], none{nullptr, nullptr};
-  hipLaunchKernelGGL((k_ns_gemm<T, SPLIT, GRAM, Src, ToPlanes>), sym, block,
-                     0, s, src, x, x, planes(w.a, SPLIT), none, ToPlanes{},
-                     r, k, step);
-  hipLaunchKernelGGL((k_ns_gemm<T, SPLIT, POLY, Src, ToPlanes>), sym, block,
-                     0, s, src, w.a, w.a, planes(w.b, SPLIT), none,
-                     ToPlanes{}, r, k, step);
+  hipLaunchKernelGGL((k_ns_gemm<SPLIT, GRAM, Src, ToPlanes>), sym, block,
+                     lds_sym, s, src, x, x, planes(w.a, SPLIT), none,
+                     ToPlanes{}, r, k, step, deep_sym);
+  hipLaunchKernelGGL((k_ns_gemm<SPLIT, POLY, Src, ToPlanes>), sym, block,
+                     lds_sym, s, src, w.a, w.a, planes(w.b, SPLIT), none,
+                     ToPlanes{}, r, k, step, deep_sym);
   if (last)
-    hipLaunchKernelGGL((k_ns_gemm<T, SPLIT, APPLY, Src, Out>), rect, block, 0,
-                       s, src, w.b, xt, none, none, out, r, k, step);
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, Out>), rect, block,
+                       lds_rect, s, src, w.b, xt, none, none, out, r, k, step,
+                       deep_rect);
   else
-    hipLaunchKernelGGL((k_ns_gemm<T, SPLIT, APPLY, Src, ToPlanes>), rect,
-                       block, 0, s, src, w.b, xt,
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, ToPlanes>), rect, block,
+                       lds_rect, s, src, w.b, xt,
                        planes(w.x[now ^ 1], next_split),
                        planes(w.xt[now ^ 1], next_split), ToPlanes{}, r, k,
-                       step);
+                       step, deep_rect);
 }
 
-template <int T, class Src, class Out>
+template <class Src, class Out>
 void ns_steps(Src src, const Work& w, int steps, int split_steps, Out out,
-              const float* r, Coef k, int64_t n_sym, int64_t n_rect,
-              hipStream_t s) {
+              const float* r, Coef k, int n_sym, int n_rect, hipStream_t s) {
   for (int i = 0; i < steps; ++i) {
-    auto f = i < split_steps ? ns_step<T, true, Src, Out>
-                             : ns_step<T, false, Src, Out>;
+    auto f = i < split_steps ? ns_step<true, Src, Out>
+                             : ns_step<false, Src, Out>;
     f(src, w, i, i + 1 < split_steps, i + 1 == steps, out, r, k, n_sym,
       n_rect, s);
   }
 }
 
+// Of `tiles` tiles of 128 x 128, how many to work on as such: two are on a
+// CU at a time, 512 on the card.  A last round of up to a quarter of that
+// ends sooner as four times as many tiles of 64 x 64.
+int64_t big_tiles(int64_t tiles) {
+  const int64_t left = tiles % 512;
+  return left <= 128 ? tiles - left : tiles;
+}
+
 template <typename T>
-void newton_schulz(const T* g, T* out, const Mat& first, int batch, int tile,
-                   int steps, int split_steps, Coef k, float eps, void* work,
+void newton_schulz(const T* g, T* out, const Mat& first, int batch, int steps,
+                   int split_steps, Coef k, float eps, void* work,
                    double* partials, float* r, hipStream_t s) {
-  const Uniform src{first, batch};
+  const int64_t nt = first.np / 64, mt = first.mp / 64;
+  const int64_t nb = nt / 2, mb = mt / 2;
+  const int64_t syms = batch * (nb * (nb + 1) / 2), rects = batch * nb * mb;
+  const int64_t big_sym = big_tiles(syms), big_rect = big_tiles(rects);
+  const Uniform src{first, batch, (int)big_sym, (int)big_rect};
   const Work w = split_work(work, (int64_t)batch * first.np * first.mp,
                             (int64_t)batch * first.np * first.np);
   hipLaunchKernelGGL(k_ns_sumsq<T>, dim3((unsigned)(batch * first.chunk1)),
                      dim3(256), 0, s, src, g, partials);
-  const int64_t packs = (int64_t)batch * (first.np / 64) * (first.mp / 64);
-  hipLaunchKernelGGL((k_ns_pack<Uniform, Plain<T>>), dim3((unsigned)packs),
-                     dim3(256), 0, s, src, Plain<T>{g}, partials,
-                     planes(w.x[0], split_steps > 0),
+  hipLaunchKernelGGL((k_ns_pack<Uniform, Plain<T>>),
+                     dim3((unsigned)(batch * nt * mt)), dim3(256), 0, s, src,
+                     Plain<T>{g}, partials, planes(w.x[0], split_steps > 0),
                      planes(w.xt[0], split_steps > 0), r, eps);
-  const int64_t nt = first.np / tile, mt = first.mp / tile;
-  auto f = tile == 64 ? ns_steps<64, Uniform, ToTensor<T>>
-                      : ns_steps<128, Uniform, ToTensor<T>>;
-  f(src, w, steps, split_steps, ToTensor<T>{out}, r, k,
-    batch * (nt * (nt + 1) / 2), batch * nt * mt, s);
+  const int64_t n_sym = big_sym + 4 * (syms - big_sym)
+                        + batch * (nt & 1 ? nt : 0);
+  const int64_t n_rect = big_rect + 4 * (rects - big_rect)
+                         + batch * ((mt & 1 ? nt : 0)
+                                    + (nt & 1 ? 2 * mb : 0));
+  ns_steps(src, w, steps, split_steps, ToTensor<T>{out}, r, k, (int)n_sym,
+           (int)n_rect, s);
 }
 
 template <typename T>
@@ -486,7 +750,7 @@ void muon_step(float* p, const T* g, float* buf, __bf16* shadow,
                const void* tables, const int64_t* layout, void* work,
                double* partials, float* r, hipStream_t s) {
   // layout: matrices, chunks, pack tiles, sym tiles, rect tiles, size of an
-  // X plane, size of an A plane, tile; the tables lie in this order
+  // X plane, size of an A plane; the tables lie in this order
   const char* at = static_cast<const char*>(tables);
   Table src;
   src.mats = reinterpret_cast<const Mat*>(at);
@@ -508,10 +772,8 @@ void muon_step(float* p, const T* g, float* buf, __bf16* shadow,
                      dim3((unsigned)layout[2]), dim3(256), 0, s, src,
                      Momentum<T>{g, buf, mu, nesterov}, partials, w.x[0],
                      w.xt[0], r, eps);
-  auto f = layout[7] == 64 ? ns_steps<64, Table, ToParams>
-                           : ns_steps<128, Table, ToParams>;
-  f(src, w, steps, steps, ToParams{p, shadow, lr, wd}, r, k, layout[3],
-    layout[4], s);
+  ns_steps(src, w, steps, steps, ToParams{p, shadow, lr, wd}, r, k,
+           (int)layout[3], (int)layout[4], s);
 }
 
 }  // namespace
@@ -522,8 +784,10 @@ extern "C" {
 
 int sgp_ns_chunk() { return CHUNK; }
 
+int64_t sgp_ns_big_tiles(int64_t tiles) { return big_tiles(tiles); }
+
 void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
-                       int batch, int tile, int steps, int split_steps,
+                       int batch, int steps, int split_steps,
                        float a, float b, float c, float growth, float eps,
                        void* work, double* partials, float* r,
                        hipStream_t s) {
@@ -531,16 +795,16 @@ void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
   const Coef k{a, b, c, log2f(growth)};
   if (dtype == 0)
     newton_schulz(static_cast<const float*>(g), static_cast<float*>(out),
-                  first, batch, tile, steps, split_steps, k, eps, work,
-                  partials, r, s);
+                  first, batch, steps, split_steps, k, eps, work, partials, r,
+                  s);
   else if (dtype == 1)
     newton_schulz(static_cast<const __bf16*>(g), static_cast<__bf16*>(out),
-                  first, batch, tile, steps, split_steps, k, eps, work,
-                  partials, r, s);
+                  first, batch, steps, split_steps, k, eps, work, partials, r,
+                  s);
   else
     newton_schulz(static_cast<const half_t*>(g), static_cast<half_t*>(out),
-                  first, batch, tile, steps, split_steps, k, eps, work,
-                  partials, r, s);
+                  first, batch, steps, split_steps, k, eps, work, partials, r,
+                  s);
 }
 
 void sgp_muon_step(int dtype, float* p, const void* g, float* buf,
