@@ -27,10 +27,11 @@
 // n and m are padded with zeros to multiples of 64, so the products have no
 // borders; zeros stay zeros in every step.
 //
-// Layout.  A plane of R rows holds 32 columns of all rows one after another,
-// then the next 32: what a tile loads of its rows for 32 of K is one
-// contiguous piece of memory, whole cache lines (rows along K would be used
-// in halves of lines).
+// Layout.  A plane holds 32 columns of all rows, then the next 32; of these
+// 16 rows at a time, as one fragment of a matrix instruction: 64 pieces of
+// 8 columns, piece l for lane l, 1 KB.  A fragment is loaded from memory or
+// LDS with neighbouring lanes at neighbouring places, and what a tile needs
+// of its rows for 32 of K is one contiguous piece of memory.
 
 #include <hip/hip_runtime.h>
 
@@ -248,9 +249,10 @@ struct Momentum {
 
 struct Planes { half_t *h, *l; };  // l may be null: hi alone
 
-// Where a plane of `rows` rows has (row, col); 32 columns are together.
+// Where a plane of `rows` rows has (row, col).
 __device__ __forceinline__ int64_t place(int row, int col, int rows) {
-  return (int64_t)(col >> 5) * rows * 32 + row * 32 + (col & 31);
+  return (int64_t)(col >> 5) * rows * 32 + (row >> 4) * 512
+         + (col >> 3 & 3) * 128 + (row & 15) * 8 + (col & 7);
 }
 
 __device__ __forceinline__ void put8(const Planes& p, int64_t i,
@@ -295,8 +297,9 @@ __global__ __launch_bounds__(256) void k_ns_pack(
   }
   __syncthreads();
   for (int k = threadIdx.x; k < 512; k += 256) {
-    // 4 neighbours have the 32 values of a row that lie together
-    const int a = (k >> 2) & 63, b = (k >> 8) * 32 + (k & 3) * 8;
+    // 16 neighbours have the same 8 columns of 16 rows
+    const int a = (k & 15) + (k >> 6 & 3) * 16;
+    const int b = (k >> 8) * 32 + (k >> 4 & 3) * 8;
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = tile[a][b + i];
@@ -323,13 +326,6 @@ __device__ __forceinline__ int x_exp(const Mat& q, float r, int step,
   return shift > 0 ? q.e - shift : q.e;
 }
 
-// Rows of 32 halves lie in LDS without padding, as the direct loads write
-// them.  Row r's four 16-byte pieces are stored in the order c ^ turn(r),
-// which spreads the 16 rows of a fragment over all banks.
-__device__ __forceinline__ int turn(int row) {
-  return ((row >> 1) & 3) ^ ((row >> 3) & 1);
-}
-
 __device__ __forceinline__ void load_lds(const half_t* from, half_t* to) {
   __builtin_amdgcn_global_load_lds(
       (const __attribute__((address_space(1))) void*)from,
@@ -350,15 +346,26 @@ struct Fragments {
   static constexpr int NP = SPLIT ? 2 : 1;
   half8 a[NP][F], b[NP][F];
   __device__ __forceinline__ void read(const half_t* lds, int plane,
-                                       int p_row, int q_row, int at) {
+                                       int p_row, int q_row, int lane) {
 #pragma unroll
     for (int x = 0; x < NP; ++x)
 #pragma unroll
       for (int i = 0; i < F; ++i) {
         a[x][i] = *reinterpret_cast<const half8*>(
-            lds + 2 * x * plane + (p_row + i * 16) * 32 + at);
+            lds + 2 * x * plane + (p_row + i * 16) * 32 + lane * 8);
         b[x][i] = *reinterpret_cast<const half8*>(
-            lds + (2 * x + 1) * plane + (q_row + i * 16) * 32 + at);
+            lds + (2 * x + 1) * plane + (q_row + i * 16) * 32 + lane * 8);
+      }
+  }
+  __device__ __forceinline__ void load(const Operands& o, int kt, int lane) {
+#pragma unroll
+    for (int x = 0; x < NP; ++x)
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        a[x][i] = *reinterpret_cast<const half8*>(
+            o.at[2 * x] + kt * o.next[0] + i * 512 + lane * 8);
+        b[x][i] = *reinterpret_cast<const half8*>(
+            o.at[2 * x + 1] + kt * o.next[1] + i * 512 + lane * 8);
       }
   }
   __device__ __forceinline__ void multiply(f32x4 (&acc)[F][F]) const {
@@ -378,23 +385,12 @@ struct Fragments {
   }
 };
 
-// Where lane l reads a fragment: row l % 16, 8 halves from 8 (l / 16).
-__device__ __forceinline__ int fragment_at(int lane) {
-  const int row = lane & 15;
-  return row * 32 + ((lane >> 4) ^ turn(row)) * 8;
-}
-// Where it loads: a direct load brings 16 rows, 4 lanes a row.
-__device__ __forceinline__ int load_at(int lane) {
-  const int row = lane >> 2;
-  return row * 32 + ((lane & 3) ^ turn(row)) * 8;
-}
-
 // One barrier: all direct loads have arrived and all reads are done.
 __device__ __forceinline__ void arrive() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-constexpr int LDS_BYTES = 65536;  // two blocks on a CU; twice that: one
+constexpr int LDS_BYTES = 65536;
 
 // 128 x 128, a wave 64 x 64 of it.  Two buffers: while one is multiplied,
 // the next 32 of K are on their way into the other.
@@ -404,16 +400,15 @@ __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
   constexpr int NP = SPLIT ? 2 : 1, PLANE = 128 * 32;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int from = load_at(lane);
   auto fetch = [&](int kt, half_t* to) {
 #pragma unroll
     for (int x = 0; x < 2 * NP; ++x)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        load_lds(o.at[x] + kt * o.next[x & 1] + (i * 4 + wave) * 512 + from,
+        load_lds(o.at[x] + kt * o.next[x & 1] + (i * 4 + wave) * 512
+                     + lane * 8,
                  to + x * PLANE + (i * 4 + wave) * 512);
   };
-  const int at = fragment_at(lane);
   const int KT = o.K / 32;
   fetch(0, lds);
   for (int kt = 0; kt < KT; ++kt) {
@@ -421,60 +416,53 @@ __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
     arrive();
     if (kt + 1 < KT) fetch(kt + 1, lds + (~kt & 1) * 2 * NP * PLANE);
     Fragments<SPLIT, 4> f;
-    f.read(now, PLANE, (wave >> 1) * 64, (wave & 1) * 64, at);
+    f.read(now, PLANE, (wave >> 1) * 64, (wave & 1) * 64, lane);
     f.multiply(acc);
   }
 }
 
-// 64 x 64, the whole of it by each wave over a quarter of K: 16 fragments
-// from 8 loads, as in the large tile, and no barrier.  A wave's loads go to
-// its own part of LDS; once its fragments are in registers the next are on
-// their way while it multiplies.  `deep`: the block has twice the LDS, and
-// a wave loads two steps ahead.
+// 64 x 64, the whole of it by each wave over a quarter of K.  A fragment is
+// 1 KB of contiguous memory, so it comes straight into registers; nothing is
+// shared between the waves before the end, and LDS, which would be the
+// bottleneck, stays out of it.  The next step's loads are on their way while
+// one is multiplied.
 template <bool SPLIT>
-__device__ __forceinline__ void product64(const Operands& o, half_t* lds,
-                                          bool deep, f32x4 (&acc)[4][4]) {
-  constexpr int NP = SPLIT ? 2 : 1, PLANE = 64 * 32, L = 8 * NP;
+__device__ __forceinline__ void product64(const Operands& o,
+                                          f32x4 (&acc)[4][4]) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  half_t* own = lds + wave * (LDS_BYTES / 8);
-  const int from = load_at(lane);
-  auto fetch = [&](int kt, half_t* to) {
-#pragma unroll
-    for (int x = 0; x < 2 * NP; ++x)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        load_lds(o.at[x] + kt * o.next[x & 1] + i * 512 + from,
-                 to + x * PLANE + i * 512);
-  };
-  const int at = fragment_at(lane);
-  const int KT = o.K / 32, ahead = deep ? 8 : 4;
-  half_t* now = own;
-  half_t* next = deep ? own + LDS_BYTES / 2 : own;
-  if (wave < KT) fetch(wave, now);
-  if (deep && wave + 4 < KT) fetch(wave + 4, next);
-  for (int kt = wave; kt < KT; kt += 4) {
-    if (deep && kt + 4 < KT)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    Fragments<SPLIT, 4> f;
-    f.read(now, PLANE, 0, 0, at);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (kt + ahead < KT) fetch(kt + ahead, now);
-    f.multiply(acc);
-    half_t* t = now;
-    now = next;
-    next = t;
+  const int KT = o.K / 32;
+  Fragments<SPLIT, 4> f[2];
+  if (wave < KT) f[0].load(o, wave, lane);
+  for (int kt = wave; kt < KT; kt += 8) {
+    if (kt + 4 < KT) f[1].load(o, kt + 4, lane);
+    f[0].multiply(acc);
+    if (kt + 4 < KT) {
+      if (kt + 8 < KT) f[0].load(o, kt + 8, lane);
+      f[1].multiply(acc);
+    }
   }
 }
 
-// Where the last product goes: a tensor, or the parameters.
+// Where the last product goes, n <= 8 values from i on: a tensor, or the
+// parameters.  8 lie at any element, in two accesses of 16 bytes.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
 template <typename T>
 struct ToTensor {
   T* out;
-  __device__ void put(int64_t i, float o, const Mat&) const {
-    out[i] = (T)o;
+  __device__ void put(int64_t i, const float* o, int n, const Mat&) const {
+    if (n >= 8) {
+      typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+      V v;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] = (T)o[x];
+      *reinterpret_cast<V*>(out + i) = v;
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x < n) out[i + x] = (T)o[x];
+    }
   }
 };
 struct ToParams {
@@ -482,11 +470,32 @@ struct ToParams {
   __bf16* shadow;
   const float* lr_ptr;
   float wd;
-  __device__ void put(int64_t i, float o, const Mat& q) const {
-    const float lr = lr_ptr[0];
-    const float v = p[i] * (1.f - lr * wd) - lr * q.scale * o;
-    p[i] = v;
-    if (shadow != nullptr) shadow[i] = (__bf16)v;
+  __device__ void put(int64_t i, const float* o, int n, const Mat& q) const {
+    const float lr = lr_ptr[0], keep = 1.f - lr * wd, step = lr * q.scale;
+    if (n >= 8) {
+      f32x4u* at = reinterpret_cast<f32x4u*>(p + i);
+      f32x4u v[2] = {at[0], at[1]};
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        v[x >> 2][x & 3] = v[x >> 2][x & 3] * keep - step * o[x];
+      at[0] = v[0];
+      at[1] = v[1];
+      if (shadow != nullptr) {
+        typedef __bf16 V __attribute__((ext_vector_type(8), aligned(2)));
+        V b;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) b[x] = (__bf16)v[x >> 2][x & 3];
+        *reinterpret_cast<V*>(shadow + i) = b;
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x < n) {
+          const float v = p[i + x] * keep - step * o[x];
+          p[i + x] = v;
+          if (shadow != nullptr) shadow[i + x] = (__bf16)v;
+        }
+    }
   }
 };
 struct ToPlanes {};  // not the last product
@@ -502,8 +511,8 @@ struct ToPlanes {};  // not the last product
 template <bool SPLIT, int MODE, class Src, class Out>
 __global__ __launch_bounds__(256, 2) void k_ns_gemm(
     Src src, Planes P, Planes Q, Planes C, Planes D, Out out,
-    const float* __restrict__ r, Coef k, int step, bool deep) {
-  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+    const float* __restrict__ r, Coef k, int step) {
+  __shared__ __attribute__((aligned(16))) char lds_raw[LDS_BYTES];
   half_t* lds = reinterpret_cast<half_t*>(lds_raw);
   float* image = reinterpret_cast<float*>(lds_raw);
   constexpr bool LAST = MODE == APPLY && !__is_same(Out, ToPlanes);
@@ -519,6 +528,8 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
                    {(int64_t)q.np * 32, (int64_t)q_rows * 32}, K};
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
+  const float rr = MODE == POLY ? 0.f : r[t.mat];
+
   f32x4 acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -527,12 +538,11 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
   if (t.big)
     product128<SPLIT>(o, lds, acc);
   else
-    product64<SPLIT>(o, lds, deep, acc);
+    product64<SPLIT>(o, acc);
 
   // what the sums are multiplied with: powers of two, and r or its square
   float f = 1.f / A_SCALE;
   if (MODE != POLY) {
-    const float rr = r[t.mat];
     const int e = x_exp(q, rr, step, k);
     if (MODE == GRAM)
       f = ldexpf(rr * rr, -2 * e) * A_SCALE;
@@ -584,20 +594,18 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
     const int rp = row0 + part * 64;  // the image's first row
     const bool mirror = MODE == APPLY ? !LAST : t.tm != t.tn;
     const bool tall = LAST && q.rows > q.cols;
-    // along rows: 4 neighbours have 32 columns, the next 4 the next row
+    // along rows: 16 neighbours have the same 8 columns of 16 rows
     if (!tall) {
       for (int u = threadIdx.x; u < 8 * W; u += 256) {
-        const int row = (u >> 2) & 63, col = (u >> 8) * 32 + (u & 3) * 8;
+        const int row = (u & 15) + (u >> 6 & 3) * 16;
+        const int col = (u >> 8) * 32 + (u >> 4 & 3) * 8;
         float v[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) v[x] = image[row * S + col + x] * f;
         if constexpr (LAST) {
           const int64_t at = q.start + (int64_t)(rp + row) * q.cols;
           if (rp + row < q.n)
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              if (col0 + col + x < q.m)
-                out.put(at + col0 + col + x, v[x], q);
+            out.put(at + col0 + col, v, q.m - col0 - col, q);
         } else if constexpr (MODE == APPLY) {
           put8(C, q.x_off + place(rp + row, col0 + col, q.np), v);
         } else {
@@ -622,8 +630,8 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
     if (mirror || tall) {
       if (MODE == POLY) __syncthreads();
       for (int u = threadIdx.x; u < 8 * W; u += 256) {
-        const int col = (u >> 2) & (W - 1);
-        const int row = (u >> (t.big ? 9 : 8)) * 32 + (u & 3) * 8;
+        const int col = (u & 15) + ((u >> 6) * 16 & (W - 1));
+        const int row = (u >> (t.big ? 9 : 8)) * 32 + (u >> 4 & 3) * 8;
         float v[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x)
@@ -631,9 +639,7 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
         if constexpr (LAST) {
           const int64_t at = q.start + (int64_t)(col0 + col) * q.cols;
           if (col0 + col < q.m)
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              if (rp + row + x < q.n) out.put(at + rp + row + x, v[x], q);
+            out.put(at + rp + row, v, q.n - rp - row, q);
         } else if constexpr (MODE == APPLY) {
           put8(D, q.x_off + place(col0 + col, rp + row, q.mp), v);
         } else {
@@ -675,27 +681,21 @@ void ns_step(Src src, const Work& w, int step, bool next_split, bool last,
              hipStream_t s) {
   const int now = step & 1;
   const dim3 block(256), sym(n_sym), rect(n_rect);
-  // a block for every CU at most: it has the CU's LDS for itself
-  const bool deep_sym = n_sym <= 256, deep_rect = n_rect <= 256;
-  const int lds_sym = deep_sym ? 2 * LDS_BYTES : LDS_BYTES;
-  const int lds_rect = deep_rect ? 2 * LDS_BYTES : LDS_BYTES;
   const Planes x = w.x[now], xt = w.xt[now], none{nullptr, nullptr};
-  hipLaunchKernelGGL((k_ns_gemm<SPLIT, GRAM, Src, ToPlanes>), sym, block,
-                     lds_sym, s, src, x, x, planes(w.a, SPLIT), none,
-                     ToPlanes{}, r, k, step, deep_sym);
-  hipLaunchKernelGGL((k_ns_gemm<SPLIT, POLY, Src, ToPlanes>), sym, block,
-                     lds_sym, s, src, w.a, w.a, planes(w.b, SPLIT), none,
-                     ToPlanes{}, r, k, step, deep_sym);
+  hipLaunchKernelGGL((k_ns_gemm<SPLIT, GRAM, Src, ToPlanes>), sym, block, 0,
+                     s, src, x, x, planes(w.a, SPLIT), none, ToPlanes{}, r, k,
+                     step);
+  hipLaunchKernelGGL((k_ns_gemm<SPLIT, POLY, Src, ToPlanes>), sym, block, 0,
+                     s, src, w.a, w.a, planes(w.b, SPLIT), none, ToPlanes{},
+                     r, k, step);
   if (last)
-    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, Out>), rect, block,
-                       lds_rect, s, src, w.b, xt, none, none, out, r, k, step,
-                       deep_rect);
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, Out>), rect, block, 0, s,
+                       src, w.b, xt, none, none, out, r, k, step);
   else
     hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, ToPlanes>), rect, block,
-                       lds_rect, s, src, w.b, xt,
-                       planes(w.x[now ^ 1], next_split),
+                       0, s, src, w.b, xt, planes(w.x[now ^ 1], next_split),
                        planes(w.xt[now ^ 1], next_split), ToPlanes{}, r, k,
-                       step, deep_rect);
+                       step);
 }
 
 template <class Src, class Out>
@@ -710,11 +710,13 @@ void ns_steps(Src src, const Work& w, int steps, int split_steps, Out out,
 }
 
 // Of `tiles` tiles of 128 x 128, how many to work on as such: two are on a
-// CU at a time, 512 on the card.  A last round of up to a quarter of that
-// ends sooner as four times as many tiles of 64 x 64.
+// CU at a time, 512 on the card.  A last round of up to three quarters of
+// that ends sooner as four times as many tiles of 64 x 64 (fp32, us: 36
+// tiles of 1000 x 2048, 485 as such and 191 as 64s; the 256 of 2048 x 2048,
+// 859 and 721).
 int64_t big_tiles(int64_t tiles) {
   const int64_t left = tiles % 512;
-  return left <= 128 ? tiles - left : tiles;
+  return left <= 384 ? tiles - left : tiles;
 }
 
 template <typename T>
