@@ -3,7 +3,9 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -124,32 +126,57 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
 
 // The tiles of one product of all matrices: X X^T or A^2 (sym: on and above
 // the diagonal) or B X.  As many 128 x 128 tiles as fill the card, the
-// longest sums first, so that what starts last ends soon.
+// longest sums first, so that what starts last ends soon; of one matrix
+// the tiles that one XCD gets (every eighth block) are neighbours.
 std::vector<Tile> product_tiles(const std::vector<Mat>& m, bool sym) {
   auto length = [&](const Tile& t) { return sym ? m[t.mat].mp : m[t.mat].np; };
-  std::vector<Tile> big, small;
-  for (int i = 0; i < (int)m.size(); ++i) {
-    const int nt = m[i].np / 64, mt = sym ? nt : m[i].mp / 64;
-    for (int tm = 0; tm < nt; ++tm)
-      for (int tn = sym ? tm : 0; tn < mt; ++tn)
-        if ((tm | 1) == nt || (tn | 1) == mt)
-          small.push_back({i, tm, tn, 0});
-        else if (!(tm & 1) && !(tn & 1))
-          big.push_back({i, tm, tn, 1});
-  }
   auto longer = [&](const Tile& x, const Tile& y) {
     return length(x) > length(y);
   };
+  std::vector<Tile> big, small;
+  for (int i = 0; i < (int)m.size(); ++i) {
+    const int nt = m[i].np / 64, mt = sym ? nt : m[i].mp / 64;
+    // four pairs of rows at a time, down before to the right
+    for (int top = 0; top < nt; top += 8)
+      for (int tn = 0; tn < mt; tn += 2)
+        for (int tm = top; tm < std::min(top + 8, nt); tm += 2) {
+          if (sym && tm > tn) continue;
+          if (tm + 1 < nt && tn + 1 < mt) {
+            big.push_back({i, tm, tn, 1});
+            continue;
+          }
+          for (int k = 0; k < 4; ++k) {
+            const Tile t{i, tm + (k & 1), tn + (k >> 1), 0};
+            if (t.tm < nt && t.tn < mt && !(sym && t.tm > t.tn))
+              small.push_back(t);
+          }
+        }
+  }
   std::stable_sort(big.begin(), big.end(), longer);
   const size_t keep = (size_t)sgp_ns_big_tiles((int64_t)big.size());
   for (size_t i = keep; i < big.size(); ++i)
     for (int k = 0; k < 4; ++k) {
-      const Tile t{big[i].mat, big[i].tm + (k >> 1), big[i].tn + (k & 1), 0};
-      if (!sym || t.tm <= t.tn) small.push_back(t);
+      const Tile t{big[i].mat, big[i].tm + (k & 1), big[i].tn + (k >> 1), 0};
+      if (!(sym && t.tm > t.tn)) small.push_back(t);
     }
   big.resize(keep);
-  std::stable_sort(small.begin(), small.end(), longer);
+  std::stable_sort(small.begin(), small.end(), [&](const Tile& x,
+                                                   const Tile& y) {
+    return length(x) != length(y) ? length(x) > length(y) : x.mat < y.mat;
+  });
   big.insert(big.end(), small.begin(), small.end());
+  for (size_t from = 0; from < big.size();) {
+    size_t to = from;
+    while (to < big.size() && big[to].mat == big[from].mat
+           && big[to].big == big[from].big)
+      ++to;
+    const std::vector<Tile> part(big.begin() + from, big.begin() + to);
+    size_t k = 0;
+    for (size_t xcd = 0; xcd < 8; ++xcd)
+      for (size_t at = from + (xcd + 8 - from % 8) % 8; at < to; at += 8)
+        big[at] = part[k++];
+    from = to;
+  }
   return big;
 }
 

@@ -166,24 +166,61 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
+// 8 values from any element on, as floats and back.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* f) {
+  typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+  for (int x = 0; x < 8; ++x) f[x] = (float)v[x];
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* f) {
+  typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  V v;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) v[x] = (T)f[x];
+  *reinterpret_cast<V*>(p) = v;
+}
+// the first n of them, 0 behind
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float* f) {
+  if (n >= 8) {
+    load8(p, f);
+  } else {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) f[x] = x < n ? (float)p[x] : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, const float* f) {
+  if (n >= 8) {
+    store8(p, f);
+  } else {
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (x < n) p[x] = (T)f[x];
+  }
+}
+
 // ------------------------------------------------------- squared norms
-// In 64 bits: squares of fp32 values leave its range, sums do not round.
-constexpr int CHUNK = 8192;
+// A block has a chunk, 8 values a thread.  Sums are in 64 bits: squares of
+// fp32 values leave its range, and the norm's error would be X's.
+constexpr int CHUNK = 2048;
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_ns_sumsq(
     Uniform src, const T* __restrict__ g, double* __restrict__ partials) {
   __shared__ double lds[4];
-  const int i = src.chunk_mat(blockIdx.x);
-  const Mat q = src.mat(i);
-  const int64_t total = (int64_t)q.rows * q.cols;
-  const int64_t from = (int64_t)(blockIdx.x - q.chunk0) * CHUNK;
-  const int64_t to = from + CHUNK < total ? from + CHUNK : total;
+  const Mat q = src.mat(src.chunk_mat(blockIdx.x));
+  const int64_t at = (int64_t)(blockIdx.x - q.chunk0) * CHUNK
+                     + threadIdx.x * 8;
+  const int64_t left = (int64_t)q.rows * q.cols - at;
+  float v[8];
+  load8(g + q.start + at, left < 8 ? (int)left : 8, v);
   double s = 0.0;
-  for (int64_t k = from + threadIdx.x; k < to; k += 256) {
-    const double v = (double)(float)g[q.start + k];
-    s += v * v;
-  }
+#pragma unroll
+  for (int x = 0; x < 8; ++x) s += (double)v[x] * v[x];
   s = block_sum(s, lds);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
@@ -202,26 +239,37 @@ __global__ __launch_bounds__(256) void k_muon_momentum(
     float wd, float rest_lr, bool nesterov, double* __restrict__ partials) {
   __shared__ double lds[4];
   const Chunk c = chunks[blockIdx.x];
-  const float lr = lr_ptr[0] * rest_lr;
-  double s = 0.0;
-  for (int k = threadIdx.x; k < c.count; k += 256) {
-    const int64_t i = c.start + k;
-    float gv = (float)g[i];
-    if (c.mat < 0) gv += wd * p[i];
-    const float b = mu * buf[i] + gv;
-    buf[i] = b;
-    const float u = nesterov ? gv + mu * b : b;
-    if (c.mat < 0) {
-      const float v = p[i] - lr * u;
-      p[i] = v;
-      if (shadow != nullptr) shadow[i] = (__bf16)v;
-    } else {
-      s += (double)u * u;
+  const int64_t i = c.start + threadIdx.x * 8;
+  const int n = c.count - (int)threadIdx.x * 8;
+  float gv[8], bv[8], u[8];
+  load8(g + i, n, gv);
+  load8(buf + i, n, bv);
+  if (c.mat >= 0) {
+    double s = 0.0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      bv[x] = mu * bv[x] + gv[x];
+      u[x] = nesterov ? gv[x] + mu * bv[x] : bv[x];
+      s += (double)u[x] * u[x];
     }
+    store8(buf + i, n, bv);
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) partials[blockIdx.x] = s;
+  } else {
+    const float lr = lr_ptr[0] * rest_lr;
+    float pv[8];
+    load8(p + i, n, pv);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      gv[x] += wd * pv[x];
+      bv[x] = mu * bv[x] + gv[x];
+      u[x] = nesterov ? gv[x] + mu * bv[x] : bv[x];
+      pv[x] -= lr * u[x];
+    }
+    store8(buf + i, n, bv);
+    store8(p + i, n, pv);
+    if (shadow != nullptr) store8(shadow + i, n, pv);
   }
-  if (c.mat < 0) return;
-  s = block_sum(s, lds);
-  if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
 // ---------------------------------------------------------------- packing
@@ -230,11 +278,13 @@ __device__ __forceinline__ half_t lo_of(float v, half_t hi) {
   return (half_t)(v - (float)hi);
 }
 
-// What the matrices are read from.
+// What the matrices are read from: the first n <= 8 values from i on.
 template <typename T>
 struct Plain {
   const T* g;
-  __device__ float at(int64_t i) const { return (float)g[i]; }
+  __device__ void read(int64_t i, int n, float* f) const {
+    load8(g + i, n, f);
+  }
 };
 template <typename T>
 struct Momentum {
@@ -242,8 +292,13 @@ struct Momentum {
   const float* buf;
   float mu;
   bool nesterov;
-  __device__ float at(int64_t i) const {
-    return nesterov ? (float)g[i] + mu * buf[i] : buf[i];
+  __device__ void read(int64_t i, int n, float* f) const {
+    load8(buf + i, n, f);
+    if (!nesterov) return;
+    float gv[8];
+    load8(g + i, n, gv);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) f[x] = gv[x] + mu * f[x];
   }
 };
 
@@ -276,6 +331,15 @@ __global__ __launch_bounds__(256) void k_ns_pack(
   __shared__ float tile[64][65];
   const Tile t = src.pack(blockIdx.x);
   const Mat q = src.mat(t.mat);
+  const bool tall = q.rows > q.cols;
+  const int a0 = (tall ? t.tn : t.tm) * 64, b0 = (tall ? t.tm : t.tn) * 64;
+  float v[2][8];
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const int a = (threadIdx.x >> 3) + y * 32, b = (threadIdx.x & 7) * 8;
+    const int n = a0 + a < q.rows ? q.cols - b0 - b : 0;
+    in.read(q.start + (int64_t)(a0 + a) * q.cols + b0 + b, n, v[y]);
+  }
   double s = 0.0;
   for (int k = q.chunk0 + threadIdx.x; k < q.chunk1; k += 256)
     s += partials[k];
@@ -285,28 +349,27 @@ __global__ __launch_bounds__(256) void k_ns_pack(
   if (t.tm == 0 && t.tn == 0 && threadIdx.x == 0)
     r_out[t.mat] = norm == 0.0 ? 0.f : (float)(norm / (norm + (double)eps));
   // tile[i][j] = X[64 tm + i][64 tn + j], read along the source's rows
-  const bool tall = q.rows > q.cols;
-  const int a0 = (tall ? t.tn : t.tm) * 64, b0 = (tall ? t.tm : t.tn) * 64;
-  for (int k = threadIdx.x; k < 4096; k += 256) {
-    const int a = k >> 6, b = k & 63;
-    float v = 0.f;
-    if (a0 + a < q.rows && b0 + b < q.cols)
-      v = (float)((double)in.at(q.start + (int64_t)(a0 + a) * q.cols + b0 + b)
-                  * inv);
-    tile[tall ? b : a][tall ? a : b] = v;
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const int a = (threadIdx.x >> 3) + y * 32, b = (threadIdx.x & 7) * 8;
+    const int n = a0 + a < q.rows ? q.cols - b0 - b : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      tile[tall ? b + i : a][tall ? a : b + i] =
+          i < n ? (float)((double)v[y][i] * inv) : 0.f;
   }
   __syncthreads();
   for (int k = threadIdx.x; k < 512; k += 256) {
     // 16 neighbours have the same 8 columns of 16 rows
     const int a = (k & 15) + (k >> 6 & 3) * 16;
     const int b = (k >> 8) * 32 + (k >> 4 & 3) * 8;
-    float v[8];
+    float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = tile[a][b + i];
-    put8(x, q.x_off + place(t.tm * 64 + a, t.tn * 64 + b, q.np), v);
+    for (int i = 0; i < 8; ++i) o[i] = tile[a][b + i];
+    put8(x, q.x_off + place(t.tm * 64 + a, t.tn * 64 + b, q.np), o);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = tile[b + i][a];
-    put8(xt, q.x_off + place(t.tn * 64 + a, t.tm * 64 + b, q.mp), v);
+    for (int i = 0; i < 8; ++i) o[i] = tile[b + i][a];
+    put8(xt, q.x_off + place(t.tn * 64 + a, t.tm * 64 + b, q.mp), o);
   }
 }
 
@@ -421,7 +484,7 @@ __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
   }
 }
 
-// 64 x 64, the whole of it by each wave over a quarter of K.  A fragment is
+// 64 x 64, the whole of it by each wave over a part of K.  A fragment is
 // 1 KB of contiguous memory, so it comes straight into registers; nothing is
 // shared between the waves before the end, and LDS, which would be the
 // bottleneck, stays out of it.  The next step's loads are on their way while
@@ -444,25 +507,13 @@ __device__ __forceinline__ void product64(const Operands& o,
   }
 }
 
-// Where the last product goes, n <= 8 values from i on: a tensor, or the
-// parameters.  8 lie at any element, in two accesses of 16 bytes.
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-
+// Where the last product goes, the first n <= 8 values from i on: a tensor,
+// or the parameters.
 template <typename T>
 struct ToTensor {
   T* out;
   __device__ void put(int64_t i, const float* o, int n, const Mat&) const {
-    if (n >= 8) {
-      typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-      V v;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] = (T)o[x];
-      *reinterpret_cast<V*>(out + i) = v;
-    } else {
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x < n) out[i + x] = (T)o[x];
-    }
+    store8(out + i, n, o);
   }
 };
 struct ToParams {
@@ -472,30 +523,12 @@ struct ToParams {
   float wd;
   __device__ void put(int64_t i, const float* o, int n, const Mat& q) const {
     const float lr = lr_ptr[0], keep = 1.f - lr * wd, step = lr * q.scale;
-    if (n >= 8) {
-      f32x4u* at = reinterpret_cast<f32x4u*>(p + i);
-      f32x4u v[2] = {at[0], at[1]};
+    float v[8];
+    load8(p + i, n, v);
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        v[x >> 2][x & 3] = v[x >> 2][x & 3] * keep - step * o[x];
-      at[0] = v[0];
-      at[1] = v[1];
-      if (shadow != nullptr) {
-        typedef __bf16 V __attribute__((ext_vector_type(8), aligned(2)));
-        V b;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) b[x] = (__bf16)v[x >> 2][x & 3];
-        *reinterpret_cast<V*>(shadow + i) = b;
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x < n) {
-          const float v = p[i + x] * keep - step * o[x];
-          p[i + x] = v;
-          if (shadow != nullptr) shadow[i + x] = (__bf16)v;
-        }
-    }
+    for (int x = 0; x < 8; ++x) v[x] = v[x] * keep - step * o[x];
+    store8(p + i, n, v);
+    if (shadow != nullptr) store8(shadow + i, n, v);
   }
 };
 struct ToPlanes {};  // not the last product
@@ -675,37 +708,39 @@ Work split_work(void* base, int64_t x_total, int64_t a_total) {
 
 Planes planes(Planes p, bool lo) { return {p.h, lo ? p.l : nullptr}; }
 
+template <bool SPLIT, int MODE, class Src, class Out>
+void product(Src src, Planes p, Planes q, Planes c, Planes d, Out out,
+             const float* r, Coef k, int step, int tiles, hipStream_t s) {
+  hipLaunchKernelGGL((k_ns_gemm<SPLIT, MODE, Src, Out>), dim3(tiles),
+                     dim3(256), 0, s, src, p, q, c, d, out, r, k, step);
+}
+
 template <bool SPLIT, class Src, class Out>
 void ns_step(Src src, const Work& w, int step, bool next_split, bool last,
-             Out out, const float* r, Coef k, int n_sym, int n_rect,
+             Out out, const float* r, Coef k, int sym, int rect,
              hipStream_t s) {
   const int now = step & 1;
-  const dim3 block(256), sym(n_sym), rect(n_rect);
   const Planes x = w.x[now], xt = w.xt[now], none{nullptr, nullptr};
-  hipLaunchKernelGGL((k_ns_gemm<SPLIT, GRAM, Src, ToPlanes>), sym, block, 0,
-                     s, src, x, x, planes(w.a, SPLIT), none, ToPlanes{}, r, k,
-                     step);
-  hipLaunchKernelGGL((k_ns_gemm<SPLIT, POLY, Src, ToPlanes>), sym, block, 0,
-                     s, src, w.a, w.a, planes(w.b, SPLIT), none, ToPlanes{},
-                     r, k, step);
+  product<SPLIT, GRAM>(src, x, x, planes(w.a, SPLIT), none, ToPlanes{}, r, k,
+                       step, sym, s);
+  product<SPLIT, POLY>(src, w.a, w.a, planes(w.b, SPLIT), none, ToPlanes{},
+                       r, k, step, sym, s);
   if (last)
-    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, Out>), rect, block, 0, s,
-                       src, w.b, xt, none, none, out, r, k, step);
+    product<SPLIT, APPLY>(src, w.b, xt, none, none, out, r, k, step, rect, s);
   else
-    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, ToPlanes>), rect, block,
-                       0, s, src, w.b, xt, planes(w.x[now ^ 1], next_split),
-                       planes(w.xt[now ^ 1], next_split), ToPlanes{}, r, k,
-                       step);
+    product<SPLIT, APPLY>(src, w.b, xt, planes(w.x[now ^ 1], next_split),
+                          planes(w.xt[now ^ 1], next_split), ToPlanes{}, r,
+                          k, step, rect, s);
 }
 
 template <class Src, class Out>
 void ns_steps(Src src, const Work& w, int steps, int split_steps, Out out,
-              const float* r, Coef k, int n_sym, int n_rect, hipStream_t s) {
+              const float* r, Coef k, int sym, int rect, hipStream_t s) {
   for (int i = 0; i < steps; ++i) {
     auto f = i < split_steps ? ns_step<true, Src, Out>
                              : ns_step<false, Src, Out>;
-    f(src, w, i, i + 1 < split_steps, i + 1 == steps, out, r, k, n_sym,
-      n_rect, s);
+    f(src, w, i, i + 1 < split_steps, i + 1 == steps, out, r, k, sym, rect,
+      s);
   }
 }
 
@@ -741,8 +776,8 @@ void newton_schulz(const T* g, T* out, const Mat& first, int batch, int steps,
   const int64_t n_rect = big_rect + 4 * (rects - big_rect)
                          + batch * ((mt & 1 ? nt : 0)
                                     + (nt & 1 ? 2 * mb : 0));
-  ns_steps(src, w, steps, split_steps, ToTensor<T>{out}, r, k, (int)n_sym,
-           (int)n_rect, s);
+  ns_steps(src, w, steps, split_steps, ToTensor<T>{out}, r, k,
+           (int)n_sym, (int)n_rect, s);
 }
 
 template <typename T>
