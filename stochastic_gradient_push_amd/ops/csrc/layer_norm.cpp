@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
@@ -25,6 +26,7 @@ void sgp_layer_norm_bwd(int dtype, const void* dy, int64_t ds, const void* x,
 
 namespace {
 
+using torch::autograd::variable_list;
 typedef torch::optional<torch::Tensor> OptTensor;
 
 int dtype_code(const torch::Tensor& x) {
@@ -169,9 +171,105 @@ layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x,
   return {dx, dres, dw, db};
 }
 
+// ------------------------------------------------------------- autograd
+// In C++: the way through the Python layer costs more than the kernels do on
+// ordinary activations.
+
+// t as a matrix of its last dimension's rows: a view where they are
+// contiguous and evenly spaced, a copy elsewhere
+torch::Tensor rows(const torch::Tensor& t) {
+  torch::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+OptTensor rows(const OptTensor& t) {
+  return t.has_value() ? OptTensor(rows(*t)) : t;
+}
+
+class LayerNorm : public torch::autograd::Function<LayerNorm> {
+ public:
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx,
+                               const torch::Tensor& x,
+                               const OptTensor& weight, const OptTensor& bias,
+                               const OptTensor& res, double eps, bool relu) {
+    auto [y, mean, rstd] = layer_norm_fwd(rows(x), weight, bias, rows(res),
+                                          eps, relu, true);
+    y = y.view(x.sizes());
+    ctx->save_for_backward({x, weight.value_or(torch::Tensor()), mean, rstd,
+                            relu ? y : torch::Tensor()});
+    const OptTensor& vector = weight.has_value() ? weight : bias;
+    int64_t flags = relu ? 1 : 0;
+    if (vector.has_value() && vector->scalar_type() == torch::kFloat32)
+      flags |= 2;
+    if (weight.has_value()) flags |= 4;
+    if (bias.has_value()) flags |= 8;
+    if (res.has_value()) flags |= 16;
+    ctx->saved_data["flags"] = flags;
+    return y;
+  }
+
+  static variable_list backward(torch::autograd::AutogradContext* ctx,
+                                variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const torch::Tensor &x = saved[0], &weight = saved[1], &mean = saved[2],
+                        &rstd = saved[3], &y = saved[4];
+    const torch::Tensor& dy = grads[0];
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    // numbered over the tensors that there are
+    size_t edge = 0;
+    auto needs = [&](bool given) {
+      return given && ctx->needs_input_grad(edge++);
+    };
+    const bool need_dx = needs(true), need_dw = needs(flags & 4),
+               need_db = needs(flags & 8), need_dres = needs(flags & 16);
+    // without a ReLU the residual's gradient is dy itself
+    const bool masked = need_dres && (flags & 1);
+    torch::Tensor dx, dw, db, dres;
+    if (need_dx || need_dw || need_db || masked) {
+      const at::AutoGradMode no_grad(false);
+      std::tie(dx, dres, dw, db) = layer_norm_bwd(
+          rows(dy), rows(x), y.defined() ? OptTensor(rows(y)) : OptTensor(),
+          weight.defined() ? OptTensor(weight) : OptTensor(), mean, rstd,
+          flags & 2, need_dx, masked, need_dw, need_db);
+      if (need_dx) dx = dx.view(x.sizes());
+      if (masked) dres = dres.view(x.sizes());
+    }
+    if (need_dres && !masked) dres = dy;
+    variable_list out = {dx, dw, db, dres, torch::Tensor(), torch::Tensor()};
+    if (!torch::GradMode::is_enabled()) return out;
+    // create_graph: these have no graph of their own, and say so when asked
+    variable_list given;
+    for (const torch::Tensor& t : out)
+      if (t.defined()) given.push_back(t.detach().requires_grad_(true));
+    if (given.empty()) return out;
+    const auto error = std::make_shared<torch::autograd::DelayedError>(
+        "layer_norm is differentiable once", (int64_t)given.size());
+    given = (*error)(std::move(given));
+    size_t k = 0;
+    for (torch::Tensor& t : out)
+      if (t.defined()) t = given[k++];
+    return out;
+  }
+};
+
+torch::Tensor layer_norm(const torch::Tensor& x, const OptTensor& weight,
+                         const OptTensor& bias, double eps,
+                         const OptTensor& res, bool relu) {
+  auto wants = [](const OptTensor& t) {
+    return t.has_value() && t->requires_grad();
+  };
+  if (torch::GradMode::is_enabled()
+      && (x.requires_grad() || wants(weight) || wants(bias) || wants(res)))
+    return LayerNorm::apply(x, weight, bias, res, eps, relu);
+  return std::get<0>(layer_norm_fwd(rows(x), weight, bias, rows(res), eps,
+                                    relu, false)).view(x.sizes());
+}
+
 }  // namespace
 
 void init_layer_norm(py::module_& m) {
+  m.def("layer_norm", &layer_norm,
+        "layer norm over the last dimension, differentiable");
   m.def("layer_norm_fwd", &layer_norm_fwd,
         "row-wise layer norm (+residual)(+ReLU) -> (y, mean, rstd)");
   m.def("layer_norm_bwd", &layer_norm_bwd,

@@ -45,19 +45,23 @@ __device__ __forceinline__ void stv(T* p, typename Pack<T>::V v) {
   *reinterpret_cast<U*>(p) = v;
 }
 
-// elements [c, c + N) of a row of C as floats, `fill` behind its end
+// elements [c, c + N) of a row of C, 0 behind its end; as they are, or as
+// floats
 template <typename T>
-__device__ __forceinline__ void load(const T* row, int c, int C, float fill,
-                                     float* f) {
+__device__ __forceinline__ typename Pack<T>::V raw(const T* row, int c,
+                                                   int C) {
   constexpr int N = Pack<T>::N;
-  if (c + N <= C) {
-    const typename Pack<T>::V v = ldv(row + c);
+  if (c + N <= C) return ldv(row + c);
+  typename Pack<T>::V v;
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = (float)v[j];
-  } else {
+  for (int j = 0; j < N; ++j) v[j] = c + j < C ? row[c + j] : (T)0.f;
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void load(const T* row, int c, int C, float* f) {
+  const typename Pack<T>::V v = raw<T>(row, c, C);
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = c + j < C ? (float)row[c + j] : fill;
-  }
+  for (int j = 0; j < Pack<T>::N; ++j) f[j] = (float)v[j];
 }
 
 template <typename T>
@@ -86,9 +90,9 @@ __device__ __forceinline__ void load_w(const void* w, bool w32, int c, int C,
   } else if (w32) {
     const float* p = static_cast<const float*>(w);
 #pragma unroll
-    for (int j = 0; j < N; j += 4) load<float>(p, c + j, C, 0.f, f + j);
+    for (int j = 0; j < N; j += 4) load<float>(p, c + j, C, f + j);
   } else {
-    load<T>(static_cast<const T*>(w), c, C, 0.f, f);
+    load<T>(static_cast<const T*>(w), c, C, f);
   }
 }
 
@@ -129,59 +133,74 @@ __device__ __forceinline__ void row_sum(float* v, float* lds) {
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 // --------------------------------------------------------------- forward
-// TPR threads hold one row, VPT 16-byte vectors each.
+// TPR threads hold one row, VPT 16-byte vectors each, and walk over the rows
+// with the weights in registers.  The next row is on its way while one is
+// reduced, where a block has only one.
 template <typename T, int TPR, int VPT>
 __global__ __launch_bounds__(block_of(TPR)) void k_ln_fwd(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ res,
     int64_t rs, const void* __restrict__ w, const void* __restrict__ b,
     bool w32, T* __restrict__ y, float* __restrict__ mean_out,
     float* __restrict__ rstd_out, float eps, int64_t M, int C, bool relu) {
+  typedef typename Pack<T>::V V;
   constexpr int N = Pack<T>::N;
   constexpr int G = block_of(TPR) / TPR;
   __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
   const int t = threadIdx.x % TPR;
-  const int g = threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t r = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
+  constexpr bool AHEAD = TPR > 64;  // shorter rows: other waves fill in
+  V next[VPT], next_res[VPT];
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (t + i * TPR) * N;
+      next[i] = raw<T>(x + row * xs, c, C);
+      if (res != nullptr) next_res[i] = raw<T>(res + row * rs, c, C);
+    }
+  };
+  if (AHEAD && r < M) fetch(r);
   float wv[VPT][N], bv[VPT][N];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     load_w<T>(w, w32, (t + i * TPR) * N, C, 1.f, wv[i]);
     load_w<T>(b, w32, (t + i * TPR) * N, C, 0.f, bv[i]);
   }
-  const float inv = 1.f / (float)C;
-  for (int64_t r = (int64_t)blockIdx.x * G + g; r < M;
-       r += (int64_t)gridDim.x * G) {
-    const T* xr = x + r * xs;
-    float f[VPT][N], s = 0.f, q = 0.f;
+  for (; r < M; r += step) {
+    V now[VPT], now_res[VPT];
+    if (!AHEAD) fetch(r);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      load<T>(xr, (t + i * TPR) * N, C, 0.f, f[i]);
-#pragma unroll
-      for (int j = 0; j < N; ++j) s += f[i][j];
+      now[i] = next[i];
+      now_res[i] = next_res[i];
     }
+    if (AHEAD && r + step < M) fetch(r + step);
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += (float)now[i][j];
     row_sum<TPR, 1>(&s, lds);
     const float mean = s / (float)C;  // exact where the sum is
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        f[i][j] -= mean;
-        if ((t + i * TPR) * N + j < C) q += f[i][j] * f[i][j];
+        const float d = (float)now[i][j] - mean;
+        if ((t + i * TPR) * N + j < C) q += d * d;
       }
     row_sum<TPR, 1>(&q, lds);
-    const float rstd = 1.f / sqrtf(q * inv + eps);
-    T* yr = y + r * C;
+    const float rstd = 1.f / sqrtf(q / (float)C + eps);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = (t + i * TPR) * N;
-      float a[N];
-      if (res != nullptr) load<T>(res + r * rs, c, C, 0.f, a);
+      float f[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        float z = f[i][j] * rstd * wv[i][j] + bv[i][j];
-        if (res != nullptr) z += a[j];
-        f[i][j] = relu && z <= 0.f ? 0.f : z;  // a NaN stays
+        float z = ((float)now[i][j] - mean) * rstd * wv[i][j] + bv[i][j];
+        if (res != nullptr) z += (float)now_res[i][j];
+        f[j] = relu && z <= 0.f ? 0.f : z;  // a NaN stays
       }
-      store<T>(yr, c, C, f[i]);
+      store<T>(y + r * C, (t + i * TPR) * N, C, f);
     }
     if (mean_out != nullptr && t == 0) {
       mean_out[r] = mean;
@@ -204,25 +223,26 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(
     const T* xr = x + r * xs;
     float f[N], s = 0.f, q = 0.f;
     for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
-      load<T>(xr, (int)c, C, 0.f, f);
+      load<T>(xr, (int)c, C, f);
 #pragma unroll
       for (int j = 0; j < N; ++j) s += f[j];
     }
     row_sum<1024, 1>(&s, lds);
     const float mean = s / (float)C;  // exact where the sum is
     for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
-      load<T>(xr, (int)c, C, mean, f);
+      load<T>(xr, (int)c, C, f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) q += (f[j] - mean) * (f[j] - mean);
+      for (int j = 0; j < N; ++j)
+        if (c + j < C) q += (f[j] - mean) * (f[j] - mean);
     }
     row_sum<1024, 1>(&q, lds);
     const float rstd = 1.f / sqrtf(q * inv + eps);
     for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
       float wv[N], bv[N], a[N];
-      load<T>(xr, (int)c, C, 0.f, f);
+      load<T>(xr, (int)c, C, f);
       load_w<T>(w, w32, (int)c, C, 1.f, wv);
       load_w<T>(b, w32, (int)c, C, 0.f, bv);
-      if (res != nullptr) load<T>(res + r * rs, (int)c, C, 0.f, a);
+      if (res != nullptr) load<T>(res + r * rs, (int)c, C, a);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         float z = (f[j] - mean) * rstd * wv[j] + bv[j];
@@ -241,21 +261,37 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(
 // -------------------------------------------------------------- backward
 // Same split.  Each thread keeps the sums of its columns over the rows of
 // its block: partials[block] = {dw[C], db[C]} in fp32, added up in a fixed
-// order by k_ln_bwd_sum.  With one block the sums are the gradients.
-template <typename T, int TPR, int VPT>
+// order by k_ln_bwd_sum.
+template <typename T, int TPR, int VPT, bool RELU>
 __global__ __launch_bounds__(block_of(TPR)) void k_ln_bwd(
     const T* __restrict__ dy, int64_t ds, const T* __restrict__ x,
     int64_t xs, const T* __restrict__ y, const void* __restrict__ w,
     bool w32, const float* __restrict__ mean, const float* __restrict__ rstd,
     T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partials,
     int64_t M, int C) {
+  typedef typename Pack<T>::V V;
   constexpr int N = Pack<T>::N;
   constexpr int BT = block_of(TPR);
   constexpr int G = BT / TPR;
   constexpr int W = BT / 64;
   __shared__ float lds[TPR > 64 ? 2 * W : W * TPR * VPT * N];
   const int t = threadIdx.x % TPR;
-  const int g = threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t r = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
+  V next_x[VPT], next_g[VPT], next_y[RELU ? VPT : 1];
+  float next_mu = 0.f, next_rs = 0.f;
+  auto fetch = [&](int64_t row) {
+    next_mu = mean[row];
+    next_rs = rstd[row];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (t + i * TPR) * N;
+      next_x[i] = raw<T>(x + row * xs, c, C);
+      next_g[i] = raw<T>(dy + row * ds, c, C);  // g = 0 behind the end
+      if (RELU) next_y[i] = raw<T>(y + row * C, c, C);
+    }
+  };
+  if (r < M) fetch(r);
   float wv[VPT][N], sw[VPT][N], sb[VPT][N];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -264,41 +300,53 @@ __global__ __launch_bounds__(block_of(TPR)) void k_ln_bwd(
     for (int j = 0; j < N; ++j) sw[i][j] = sb[i][j] = 0.f;
   }
   const float inv = 1.f / (float)C;
-  for (int64_t r = (int64_t)blockIdx.x * G + g; r < M;
-       r += (int64_t)gridDim.x * G) {
-    const float mu = mean[r], rs = rstd[r];
-    float h[VPT][N], gv[VPT][N], s[2] = {0.f, 0.f};
+  for (; r < M; r += step) {
+    V xv[VPT], gv[VPT];
+    const float mu = next_mu, rs = next_rs;
+    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = (t + i * TPR) * N;
-      load<T>(x + r * xs, c, C, mu, h[i]);  // hat = 0 behind the end
-      load<T>(dy + r * ds, c, C, 0.f, gv[i]);
-      if (y != nullptr) {
-        float a[N];
-        load<T>(y + r * C, c, C, 0.f, a);
+      xv[i] = next_x[i];
+      gv[i] = next_g[i];
+      if constexpr (RELU)
 #pragma unroll
-        for (int j = 0; j < N; ++j) gv[i][j] = a[j] <= 0.f ? 0.f : gv[i][j];
-      }
-      if (dres != nullptr) store<T>(dres + r * C, c, C, gv[i]);
+        for (int j = 0; j < N; ++j)
+          if ((float)next_y[i][j] <= 0.f) gv[i][j] = (T)0.f;
+      if (dres != nullptr) {
+        const int c = (t + i * TPR) * N;
+        if (c + N <= C) {
+          stv(dres + r * C + c, gv[i]);
+        } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        h[i][j] = (h[i][j] - mu) * rs;
-        sw[i][j] += gv[i][j] * h[i][j];
-        sb[i][j] += gv[i][j];
-        gv[i][j] *= wv[i][j];
-        s[0] += gv[i][j];
-        s[1] += gv[i][j] * h[i][j];
+          for (int j = 0; j < N; ++j)
+            if (c + j < C) dres[r * C + c + j] = gv[i][j];
+        }
       }
     }
+    if (r + step < M) fetch(r + step);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float g = (float)gv[i][j], h = ((float)xv[i][j] - mu) * rs;
+        sw[i][j] += g * h;
+        sb[i][j] += g;
+        const float gw = g * wv[i][j];
+        s[0] += gw;
+        s[1] += gw * h;
+      }
     if (dx != nullptr) {
       row_sum<TPR, 2>(s, lds);
       const float m0 = s[0] * inv, m1 = s[1] * inv;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
+        float f[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          gv[i][j] = rs * (gv[i][j] - m0 - h[i][j] * m1);
-        store<T>(dx + r * C, (t + i * TPR) * N, C, gv[i]);
+        for (int j = 0; j < N; ++j) {
+          const float h = ((float)xv[i][j] - mu) * rs;
+          f[j] = rs * ((float)gv[i][j] * wv[i][j] - m0 - h * m1);
+        }
+        store<T>(dx + r * C, (t + i * TPR) * N, C, f);
       }
     }
   }
@@ -352,12 +400,12 @@ __global__ __launch_bounds__(1024) void k_ln_bwd_long(
       float s[2] = {0.f, 0.f};
       for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
         float h[N], gv[N], wv[N];
-        load<T>(x + r * xs, (int)c, C, mu, h);
-        load<T>(dy + r * ds, (int)c, C, 0.f, gv);
+        load<T>(x + r * xs, (int)c, C, h);
+        load<T>(dy + r * ds, (int)c, C, gv);
         load_w<T>(w, w32, (int)c, C, 1.f, wv);
         if (y != nullptr) {
           float a[N];
-          load<T>(y + r * C, (int)c, C, 0.f, a);
+          load<T>(y + r * C, (int)c, C, a);
 #pragma unroll
           for (int j = 0; j < N; ++j) gv[j] = a[j] <= 0.f ? 0.f : gv[j];
         }
@@ -398,11 +446,11 @@ __global__ __launch_bounds__(256) void k_ln_bwd_cols(
   for (int64_t r = blockIdx.y; r < M; r += gridDim.y) {
     const float mu = mean[r], rs = rstd[r];
     float h[N], gv[N];
-    load<T>(x + r * xs, c, C, mu, h);
-    load<T>(dy + r * ds, c, C, 0.f, gv);
+    load<T>(x + r * xs, c, C, h);
+    load<T>(dy + r * ds, c, C, gv);
     if (y != nullptr) {
       float a[N];
-      load<T>(y + r * C, c, C, 0.f, a);
+      load<T>(y + r * C, c, C, a);
 #pragma unroll
       for (int j = 0; j < N; ++j) gv[j] = a[j] <= 0.f ? 0.f : gv[j];
     }
@@ -421,23 +469,37 @@ __global__ __launch_bounds__(256) void k_ln_bwd_cols(
     }
 }
 
-// Column sums of partials [P][2C]: a block has 16 columns, 16 threads on
-// each, which add up in a fixed order.
+// Column sums of partials [P][2C]: a block has 16 columns and `blockDim.x`
+// / 16 threads on each, which add up in a fixed order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_ln_bwd_sum(
+__global__ __launch_bounds__(1024) void k_ln_bwd_sum(
     const float* __restrict__ partials, int P, int C, void* __restrict__ dw,
     void* __restrict__ db, bool w32) {
-  __shared__ float lds[256];
+  __shared__ float lds[1024];
   const int cl = threadIdx.x & 15, k0 = threadIdx.x >> 4;
-  const int64_t c = (int64_t)blockIdx.x * 16 + cl;
+  const int K = blockDim.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + cl, S = 2 * (int64_t)C;
   float v = 0.f;
-  if (c < 2 * (int64_t)C)
-    for (int k = k0; k < P; k += 16) v += partials[(int64_t)k * 2 * C + c];
+  if (c < S) {
+    const float* p = partials + c;
+    int k = k0;
+    for (; k + 7 * K < P; k += 8 * K) {  // eight on their way at once
+      float a[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = p[(int64_t)(k + i * K) * S];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += a[i];
+    }
+    for (; k < P; k += K) v += p[(int64_t)k * S];
+  }
   lds[threadIdx.x] = v;
   __syncthreads();
-  if (k0 != 0 || c >= 2 * (int64_t)C) return;
-#pragma unroll
-  for (int k = 1; k < 16; ++k) v += lds[k * 16 + cl];
+  for (int h = K / 2; h > 0; h >>= 1) {
+    if (k0 < h) lds[threadIdx.x] += lds[threadIdx.x + h * 16];
+    __syncthreads();
+  }
+  if (k0 != 0 || c >= S) return;
+  v = lds[cl];
   if (c < C) {
     if (dw != nullptr) put_w<T>(dw, w32, c, v);
   } else if (db != nullptr) {
@@ -447,8 +509,9 @@ __global__ __launch_bounds__(256) void k_ln_bwd_sum(
 
 // ---------------------------------------------------------------- launch
 // The narrowest row group that holds a row in registers: short rows share
-// a wave, rows of up to 256 vectors have one, longer ones a block.
-constexpr int MAX_VECTORS = 1024 * 4;
+// a wave, longer ones have a wave or a block.  Two vectors a thread at most:
+// with four, the backward pass has 200 registers and more, and spills.
+constexpr int MAX_VECTORS = 1024 * 2;
 
 #define LN_FOR_SHAPE(nv, CALL)                                     \
   do {                                                             \
@@ -457,11 +520,10 @@ constexpr int MAX_VECTORS = 1024 * 4;
     else if ((nv) <= 32) { CALL(32, 1); }                          \
     else if ((nv) <= 64) { CALL(64, 1); }                          \
     else if ((nv) <= 128) { CALL(64, 2); }                         \
-    else if ((nv) <= 256) { CALL(64, 4); }                         \
+    else if ((nv) <= 256) { CALL(256, 1); }                        \
     else if ((nv) <= 512) { CALL(256, 2); }                        \
-    else if ((nv) <= 1024) { CALL(256, 4); }                       \
-    else if ((nv) <= 2048) { CALL(512, 4); }                       \
-    else { CALL(1024, 4); }                                        \
+    else if ((nv) <= 1024) { CALL(512, 2); }                       \
+    else { CALL(1024, 2); }                                        \
   } while (0)
 
 template <typename T>
@@ -470,10 +532,22 @@ int vectors(int64_t C) {
 }
 
 int groups_of(int nv) {  // rows that a block of k_ln_fwd / k_ln_bwd has
-  return nv <= 8 ? 32 : nv <= 16 ? 16 : nv <= 32 ? 8 : nv <= 256 ? 4 : 1;
+  return nv <= 8 ? 32 : nv <= 16 ? 16 : nv <= 32 ? 8 : nv <= 128 ? 4 : 1;
 }
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Blocks that the card holds at once.  A forward grid has no more: its
+// blocks walk over the rows and read the weights once.
+template <class K>
+int64_t resident(K kernel, int threads) {
+  int per_cu = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(
+          &per_cu, reinterpret_cast<const void*>(kernel), threads, 0)
+          != hipSuccess || per_cu < 1)
+    per_cu = 1;
+  return 256 * (int64_t)per_cu;
+}
 
 template <typename T>
 void fwd(const void* x, int64_t xs, const void* res, int64_t rs,
@@ -491,21 +565,39 @@ void fwd(const void* x, int64_t xs, const void* res, int64_t rs,
                        relu);
     return;
   }
-  int64_t grid = cdiv(M, groups_of(nv));
-  if (grid > 2048) grid = 2048;
+  const int64_t rows = cdiv(M, groups_of(nv));
 #define LN_FWD(TPR, VPT)                                              \
-  hipLaunchKernelGGL((k_ln_fwd<T, TPR, VPT>), dim3((unsigned)grid),   \
+  static const int64_t most =                                         \
+      resident(k_ln_fwd<T, TPR, VPT>, block_of(TPR));                 \
+  hipLaunchKernelGGL((k_ln_fwd<T, TPR, VPT>),                         \
+                     dim3((unsigned)(rows < most ? rows : most)),     \
                      dim3(block_of(TPR)), 0, s, xp, xs, rp, rs, w, b, \
                      w32, yp, mean, rstd, eps, M, C, relu)
   LN_FOR_SHAPE(nv, LN_FWD);
 #undef LN_FWD
 }
 
+// Blocks of the backward pass, each with a row of partial sums: what the
+// card holds at once, if the partial sums (16 bytes a column, written and
+// read) then stay below a quarter of the rows (x, dy and dx); two a CU, one
+// of 1024 threads, in any case.
 template <typename T>
 int partial_rows(int64_t M, int C) {
   const int nv = vectors<T>(C);
-  int64_t p = nv > MAX_VECTORS ? cdiv(M, 16) : cdiv(M, groups_of(nv));
-  return (int)(p < 512 ? p : 512);
+  if (nv > MAX_VECTORS) return (int)(cdiv(M, 16) < 512 ? cdiv(M, 16) : 512);
+  int64_t most = 0;
+#define LN_MOST(TPR, VPT)                                             \
+  static const int64_t n =                                            \
+      resident(k_ln_bwd<T, TPR, VPT, true>, block_of(TPR));                 \
+  most = n
+  LN_FOR_SHAPE(nv, LN_MOST);
+#undef LN_MOST
+  const int64_t least = nv > 1024 ? 256 : 512;
+  const int64_t small = M * (int64_t)sizeof(T) * 3 / 64;
+  if (most > small) most = small;
+  if (most < least) most = least;
+  const int64_t rows = cdiv(M, groups_of(nv));
+  return (int)(rows < most ? rows : most);
 }
 
 template <typename T>
@@ -533,16 +625,19 @@ void bwd(const void* dy, int64_t ds, const void* x, int64_t xs,
     }
   } else {
 #define LN_BWD(TPR, VPT)                                              \
-  hipLaunchKernelGGL((k_ln_bwd<T, TPR, VPT>), dim3(P),                \
-                     dim3(block_of(TPR)), 0, s, dp, ds, xp, xs, yp,   \
-                     w, w32, mean, rstd, dxp, drp, partials, M, C)
+  auto f = yp != nullptr ? k_ln_bwd<T, TPR, VPT, true>                \
+                         : k_ln_bwd<T, TPR, VPT, false>;              \
+  hipLaunchKernelGGL(f, dim3(P), dim3(block_of(TPR)), 0, s, dp, ds,   \
+                     xp, xs, yp, w, w32, mean, rstd, dxp, drp,        \
+                     partials, M, C)
     LN_FOR_SHAPE(nv, LN_BWD);
 #undef LN_BWD
   }
   if (partials != nullptr)
     hipLaunchKernelGGL(k_ln_bwd_sum<T>,
-                       dim3((unsigned)cdiv(2 * (int64_t)C, 16)), dim3(256),
-                       0, s, partials, P, C, dw, db, g32);
+                       dim3((unsigned)cdiv(2 * (int64_t)C, 16)),
+                       dim3(P > 64 ? 1024 : 256), 0, s, partials, P, C, dw,
+                       db, g32);
 }
 
 }  // namespace

@@ -9,58 +9,8 @@ that gossip leaves different from rank to rank.
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as a matrix of its last dimension's rows.  A view where the
-    rows are contiguous and evenly spaced, a copy elsewhere."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
-
-
-class _LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, eps, relu):
-        from . import _ext_for
-
-        x2d = _rows(x)
-        y, mean, rstd = _ext_for(x).layer_norm_fwd(
-            x2d, weight, bias, None if residual is None else _rows(residual),
-            eps, relu, True,
-        )
-        y = y.view(x.shape)
-        ctx.save_for_backward(x, weight, mean, rstd, y if relu else None)
-        vector = weight if weight is not None else bias
-        ctx.vectors_fp32 = (
-            vector is not None and vector.dtype == torch.float32
-        )
-        ctx.relu = relu
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        from . import _ext_for
-
-        x, weight, mean, rstd, y = ctx.saved_tensors
-        need_dx, need_dw, need_db, need_dres = ctx.needs_input_grad[:4]
-        dx = dw = db = dres = None
-        # without a ReLU the residual's gradient is dy itself
-        masked = need_dres and ctx.relu
-        if need_dx or need_dw or need_db or masked:
-            dx, dres, dw, db = _ext_for(x).layer_norm_bwd(
-                _rows(dy), _rows(x), None if y is None else _rows(y), weight,
-                mean, rstd, ctx.vectors_fp32, need_dx, masked, need_dw,
-                need_db,
-            )
-            dx = dx.view(x.shape) if need_dx else None
-            dres = dres.view(x.shape) if masked else None
-        if need_dres and not masked:
-            dres = dy
-        return dx, dw, db, dres, None, None
 
 
 def layer_norm(
@@ -125,18 +75,9 @@ def layer_norm(
             y = y + residual.float()
         return (torch.relu(y) if relu else y).to(x.dtype)
 
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad
-        for t in (x, weight, bias, residual)
-    ):
-        return _LayerNormFn.apply(x, weight, bias, residual, float(eps),
-                                  bool(relu))
     from . import _ext_for
 
-    y, _, _ = _ext_for(x).layer_norm_fwd(
-        _rows(x), weight, bias, None if residual is None else _rows(residual),
-        eps, relu, False,
+    return _ext_for(x).layer_norm(
+        x, weight if weight is None else weight.contiguous(),
+        bias if bias is None else bias.contiguous(), eps, residual, relu,
     )
-    return y.view(x.shape)
