@@ -15,6 +15,7 @@
 extern "C" {
 int sgp_ns_chunk();
 int64_t sgp_ns_big_tiles(int64_t tiles);
+bool sgp_ns_is_small(int n, int m);
 void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
                        int batch, int steps, int split_steps, float a,
                        float b, float c, float growth, float eps,
@@ -109,16 +110,20 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
   TORCH_CHECK(x_total / 4096 < (int64_t(1) << 31)
               && batch * q.chunk1 < (int64_t(1) << 31),
               "newton_schulz: too many values in one call");
-  const auto opt = g.options();
-  torch::Tensor work = torch::empty({work_size(x_total, a_total)},
-                                    opt.dtype(torch::kFloat16));
-  torch::Tensor partials = torch::empty({batch * q.chunk1},
-                                        opt.dtype(torch::kFloat64));
-  torch::Tensor r = torch::empty({batch}, opt.dtype(torch::kFloat32));
+  torch::Tensor work, partials, r;
+  if (!sgp_ns_is_small(q.n, q.m)) {
+    const auto opt = g.options();
+    work = torch::empty({work_size(x_total, a_total)},
+                        opt.dtype(torch::kFloat16));
+    partials = torch::empty({batch * q.chunk1}, opt.dtype(torch::kFloat64));
+    r = torch::empty({batch}, opt.dtype(torch::kFloat32));
+  }
   sgp_newton_schulz(dtype, g.data_ptr(), out.data_ptr(), &q, (int)batch,
                     (int)steps, (int)split_steps, (float)a, (float)b,
-                    (float)c, (float)growth, (float)eps, work.data_ptr(),
-                    partials.data_ptr<double>(), r.data_ptr<float>(),
+                    (float)c, (float)growth, (float)eps,
+                    work.defined() ? work.data_ptr() : nullptr,
+                    work.defined() ? partials.data_ptr<double>() : nullptr,
+                    work.defined() ? r.data_ptr<float>() : nullptr,
                     stream_of(g));
   C10_HIP_CHECK(hipGetLastError());
   return out;

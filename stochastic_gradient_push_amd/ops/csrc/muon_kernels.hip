@@ -431,56 +431,85 @@ struct Fragments {
             o.at[2 * x + 1] + kt * o.next[1] + i * 512 + lane * 8);
       }
   }
+  // the three products of a pair one after another for all fragments: a
+  // matrix instruction that adds to the sum of the one before waits for it
   __device__ __forceinline__ void multiply(f32x4 (&acc)[F][F]) const {
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+    for (int x = 0; x < (SPLIT ? 3 : 1); ++x)
 #pragma unroll
-      for (int j = 0; j < F; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            a[0][i], b[0][j], acc[i][j], 0, 0, 0);
-        if (SPLIT) {
+      for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              a[0][i], b[NP - 1][j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              a[NP - 1][i], b[0][j], acc[i][j], 0, 0, 0);
-        }
-      }
+              a[x == 2 ? NP - 1 : 0][i], b[x == 1 ? NP - 1 : 0][j],
+              acc[i][j], 0, 0, 0);
   }
 };
 
-// One barrier: all direct loads have arrived and all reads are done.
+// Everything but the newest N direct loads has arrived, for every wave, and
+// every wave is done with what it read before.
+template <int N>
 __device__ __forceinline__ void arrive() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N)
+               : "memory");
 }
 
-constexpr int LDS_BYTES = 65536;
+constexpr int LDS_BYTES = 65536;  // two blocks on a CU
 
-// 128 x 128, a wave 64 x 64 of it.  Two buffers: while one is multiplied,
-// the next 32 of K are on their way into the other.
+// 128 x 128, a wave 64 x 64 of it, 32 of K at a time.  K goes through S
+// buffers: while one is multiplied, the next S - 1 are on their way.
 template <bool SPLIT>
 __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
                                            f32x4 (&acc)[4][4]) {
   constexpr int NP = SPLIT ? 2 : 1, PLANE = 128 * 32;
+  constexpr int S = LDS_BYTES / (2 * NP * PLANE * 2);
+  constexpr int L = 4 * NP;         // direct loads of a wave for 32 of K
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  auto fetch = [&](int kt, half_t* to) {
+  auto fetch = [&](int kt, int buf) {
 #pragma unroll
     for (int x = 0; x < 2 * NP; ++x)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         load_lds(o.at[x] + kt * o.next[x & 1] + (i * 4 + wave) * 512
                      + lane * 8,
-                 to + x * PLANE + (i * 4 + wave) * 512);
+                 lds + (buf * 2 * NP + x) * PLANE + (i * 4 + wave) * 512);
   };
-  const int KT = o.K / 32;
-  fetch(0, lds);
-  for (int kt = 0; kt < KT; ++kt) {
-    half_t* now = lds + (kt & 1) * 2 * NP * PLANE;
-    arrive();
-    if (kt + 1 < KT) fetch(kt + 1, lds + (~kt & 1) * 2 * NP * PLANE);
-    Fragments<SPLIT, 4> f;
-    f.read(now, PLANE, (wave >> 1) * 64, (wave & 1) * 64, lane);
-    f.multiply(acc);
+  auto read = [&](Fragments<SPLIT, 4>& f, int buf) {
+    f.read(lds + buf * 2 * NP * PLANE, PLANE, (wave >> 1) * 64,
+           (wave & 1) * 64, lane);
+  };
+  const int KT = o.K / 32;  // even
+#pragma unroll
+  for (int kt = 0; kt < S; ++kt)
+    if (kt < KT) fetch(kt, kt);
+  Fragments<SPLIT, 4> f[2];
+  if (KT >= S)
+    arrive<(S - 1) * L>();
+  else
+    arrive<0>();
+  read(f[0], 0);
+  int buf = 0;  // of f[0]
+  for (int kt = 0; kt < KT; kt += 2) {
+    // f[0] has kt; kt + 1 is read and kt + S fetched while it is multiplied
+    if (kt + S <= KT)
+      arrive<(S - 2) * L>();
+    else
+      arrive<0>();
+    const int b1 = buf + 1 == S ? 0 : buf + 1;
+    read(f[1], b1);
+    if (kt + S < KT) fetch(kt + S, buf);
+    f[0].multiply(acc);
+    buf = b1 + 1 == S ? 0 : b1 + 1;
+    if (kt + 2 < KT) {
+      if (kt + 1 + S <= KT)
+        arrive<(S - 2) * L>();
+      else
+        arrive<0>();
+      read(f[0], buf);
+      if (kt + 1 + S < KT) fetch(kt + 1 + S, b1);
+    }
+    f[1].multiply(acc);
   }
 }
 
@@ -683,6 +712,189 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
   }
 }
 
+// ---------------------------------------------------------- small matrices
+// n <= 64 and m <= 192: one block does all steps of a matrix, with X, its
+// transpose, A and B in LDS, where 15 launches would each wait for a few
+// microseconds.  The planes are those of the large products, padded to 64
+// rows; a wave has 16 rows of every result.
+constexpr int SMALL_N = 64, SMALL_M = 192;
+
+// acc[j] += rows [16 wave, 16 wave + 16) of P times rows [16 j, 16 j + 16) of
+// the R rows of Q, over K.
+template <bool SPLIT, int R, int K>
+__device__ __forceinline__ void small_product(const half_t* p, int p_plane,
+                                              const half_t* q, int q_plane,
+                                              int wave, int lane,
+                                              f32x4* acc) {
+#pragma unroll
+  for (int k0 = 0; k0 < K; k0 += 32) {
+    const half_t* pa = p + k0 * SMALL_N + wave * 512 + lane * 8;
+    const half_t* qa = q + k0 * R + lane * 8;
+    half8 a[2], b[2][R / 16];
+#pragma unroll
+    for (int x = 0; x < (SPLIT ? 2 : 1); ++x) {
+      a[x] = *reinterpret_cast<const half8*>(pa + x * p_plane);
+#pragma unroll
+      for (int j = 0; j < R / 16; ++j)
+        b[x][j] = *reinterpret_cast<const half8*>(qa + x * q_plane + j * 512);
+    }
+#pragma unroll
+    for (int x = 0; x < (SPLIT ? 3 : 1); ++x)
+#pragma unroll
+      for (int j = 0; j < R / 16; ++j)
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            a[x == 2], b[x == 1][j], acc[j], 0, 0, 0);
+  }
+}
+
+// 4 values that lie together, as pairs.
+__device__ __forceinline__ void put4(half_t* h, int plane, const float* v) {
+  half4 hi, lo;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    hi[x] = hi_of(v[x]);
+    lo[x] = lo_of(v[x], hi[x]);
+  }
+  *reinterpret_cast<half4*>(h) = hi;
+  *reinterpret_cast<half4*>(h + plane) = lo;
+}
+
+// One step on the planes in LDS; the result in `acc`, not scaled.
+template <bool SPLIT, int MP>
+__device__ __forceinline__ void small_step(const half_t* x, const half_t* xt,
+                                           half_t* a, half_t* b, float gram,
+                                           const Coef& k, f32x4* acc) {
+  constexpr int XP = SMALL_N * MP, AP = SMALL_N * SMALL_N;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r0 = wave * 16 + (lane >> 4) * 4;  // this lane's 4 rows
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // A and B are symmetric: a lane's 4 rows of a column are stored as 4
+  // columns of a row, which lie together
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = zero;
+  small_product<SPLIT, SMALL_N, MP>(x, XP, x, XP, wave, lane, acc);
+  float av[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) av[j][i] = acc[j][i] * gram;
+    put4(a + place(j * 16 + (lane & 15), r0, SMALL_N), AP, av[j]);
+    acc[j] = zero;
+  }
+  __syncthreads();
+  small_product<SPLIT, SMALL_N, SMALL_N>(a, AP, a, AP, wave, lane, acc);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int col = j * 16 + (lane & 15);
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = (k.b * av[j][i] + k.c * acc[j][i] * (1.f / A_SCALE))
+             * (B_SCALE / A_SCALE) + (r0 + i == col ? k.a * B_SCALE : 0.f);
+    put4(b + place(col, r0, SMALL_N), AP, v);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < MP / 16; ++j) acc[j] = zero;
+  small_product<SPLIT, MP, SMALL_N>(b, AP, xt, XP, wave, lane, acc);
+  __syncthreads();
+}
+
+template <typename T, int MP>
+__global__ __launch_bounds__(256) void k_ns_small(
+    Uniform src, const T* __restrict__ g, T* __restrict__ out, int steps,
+    int split_steps, Coef k, float eps) {
+  constexpr int XP = SMALL_N * MP, AP = SMALL_N * SMALL_N;
+  constexpr int V = XP / 2048;  // 8 values at a time a thread
+  __shared__ __attribute__((aligned(16))) half_t x[2 * XP], xt[2 * XP],
+      a[2 * AP], b[2 * AP];
+  const Mat q = src.mat(blockIdx.x);
+  const bool tall = q.rows > q.cols;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int total = q.rows * q.cols;
+
+  float v[V][8];
+  double s = 0.0;
+#pragma unroll
+  for (int y = 0; y < V; ++y) {
+    const int i = (y * 256 + threadIdx.x) * 8;
+    load8(g + q.start + i, total - i, v[y]);
+  }
+#pragma unroll
+  for (int i = threadIdx.x * 8; i < 2 * XP; i += 2048) {
+    const half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    *reinterpret_cast<half8*>(x + i) = zero;
+    *reinterpret_cast<half8*>(xt + i) = zero;
+  }
+#pragma unroll
+  for (int y = 0; y < V; ++y)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += (double)v[y][i] * v[y][i];
+  const double norm = sqrt(block_sum(s, reinterpret_cast<double*>(a)));
+  const double inv = norm == 0.0 ? 0.0 : ldexp(1.0 / norm, q.e);
+  const float r = norm == 0.0 ? 0.f : (float)(norm / (norm + (double)eps));
+#pragma unroll
+  for (int y = 0; y < V; ++y) {
+    const int first = (y * 256 + threadIdx.x) * 8;
+    int row = first / q.cols, col = first % q.cols;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (first + i < total) {
+        const float f = (float)((double)v[y][i] * inv);
+        const half_t h = hi_of(f), l = lo_of(f, h);
+        const int xr = tall ? col : row, xc = tall ? row : col;
+        const int at = (int)place(xr, xc, SMALL_N), to = (int)place(xc, xr, MP);
+        x[at] = h;
+        x[at + XP] = l;
+        xt[to] = h;
+        xt[to + XP] = l;
+      }
+      if (++col == q.cols) {
+        col = 0;
+        ++row;
+      }
+    }
+  }
+  __syncthreads();
+
+  f32x4 acc[MP / 16];
+  const int r0 = wave * 16 + (lane >> 4) * 4;
+  for (int step = 0; step < steps; ++step) {
+    const int e = x_exp(q, r, step, k);
+    const float gram = ldexpf(r * r, -2 * e) * A_SCALE;
+    if (step < split_steps)
+      small_step<true, MP>(x, xt, a, b, gram, k, acc);
+    else
+      small_step<false, MP>(x, xt, a, b, gram, k, acc);
+    const bool last = step + 1 == steps;
+    const float f = last ? ldexpf(r / B_SCALE, -e)
+                         : ldexpf(1.f / B_SCALE, x_exp(q, r, step + 1, k) - e);
+#pragma unroll
+    for (int j = 0; j < MP / 16; ++j) {
+      const int col = j * 16 + (lane & 15);
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = acc[j][i] * f;
+      if (last) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r0 + i < q.n && col < q.m)
+            out[q.start + (tall ? col * q.cols + r0 + i
+                                : (r0 + i) * q.cols + col)] = (T)w[i];
+      } else {
+        put4(xt + place(col, r0, MP), XP, w);
+        half_t* to = x + place(r0, col, SMALL_N);  // a row: 8 further
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          to[i * 8] = hi_of(w[i]);
+          to[i * 8 + XP] = lo_of(w[i], hi_of(w[i]));
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
 // Workspace, in fp16 values: X and its transpose twice, A and B, each as
 // two planes; x_total and a_total: the sizes of one plane.
 struct Work {
@@ -754,10 +966,21 @@ int64_t big_tiles(int64_t tiles) {
   return left <= 384 ? tiles - left : tiles;
 }
 
+// Such a matrix needs no workspace.
+bool is_small(int n, int m) { return n <= SMALL_N && m <= SMALL_M; }
+
 template <typename T>
 void newton_schulz(const T* g, T* out, const Mat& first, int batch, int steps,
                    int split_steps, Coef k, float eps, void* work,
                    double* partials, float* r, hipStream_t s) {
+  if (is_small(first.n, first.m)) {
+    const Uniform src{first, batch, 0, 0};
+    auto f = first.mp == 64 ? k_ns_small<T, 64>
+             : first.mp == 128 ? k_ns_small<T, 128> : k_ns_small<T, 192>;
+    hipLaunchKernelGGL(f, dim3((unsigned)batch), dim3(256), 0, s, src, g, out,
+                       steps, split_steps, k, eps);
+    return;
+  }
   const int64_t nt = first.np / 64, mt = first.mp / 64;
   const int64_t nb = nt / 2, mb = mt / 2;
   const int64_t syms = batch * (nb * (nb + 1) / 2), rects = batch * nb * mb;
@@ -822,6 +1045,8 @@ extern "C" {
 int sgp_ns_chunk() { return CHUNK; }
 
 int64_t sgp_ns_big_tiles(int64_t tiles) { return big_tiles(tiles); }
+
+bool sgp_ns_is_small(int n, int m) { return is_small(n, m); }
 
 void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
                        int batch, int steps, int split_steps,

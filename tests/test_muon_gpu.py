@@ -59,9 +59,10 @@ def strong(rows, cols, seed=0, batch=()):
         randn(*batch, rows, k), randn(*batch, k, cols))
 
 
-# both tiles, their borders, both orientations
+# one block's, both tiles, their borders, both orientations
 SHAPES = [(1, 1), (1, 9), (7, 1), (3, 2), (16, 16), (63, 65), (64, 64),
-          (65, 64), (64, 576), (640, 40), (129, 257), (256, 256), (257, 300),
+          (65, 64), (65, 65), (64, 192), (64, 193), (192, 33), (193, 33),
+          (20, 129), (64, 576), (640, 40), (129, 257), (256, 256), (257, 300),
           (300, 1000), (1000, 260), (512, 512), (385, 385)]
 
 
