@@ -39,6 +39,10 @@ struct Mat {
   float scale;
 };
 struct Tile { int mat, tm, tn, big; };
+struct Task {
+  Mat q;
+  Tile t;
+};
 struct Chunk { int64_t start; int count, mat; };
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -196,7 +200,7 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
   const int chunk = sgp_ns_chunk();
   std::vector<Mat> m;
   std::vector<Chunk> chunks;
-  std::vector<Tile> packs, syms, rects;
+  std::vector<Tile> pack_tiles;
   std::vector<std::pair<int64_t, int64_t>> taken;
   int64_t x_total = 0, a_total = 0;
   for (const auto& [start, rows, cols, scale] : mats) {
@@ -214,12 +218,19 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
     x_total += q.np * (int64_t)q.mp;
     a_total += q.np * (int64_t)q.np;
     for (int tm = 0; tm < q.np / 64; ++tm)
-      for (int tn = 0; tn < q.mp / 64; ++tn) packs.push_back({i, tm, tn, 0});
+      for (int tn = 0; tn < q.mp / 64; ++tn)
+        pack_tiles.push_back({i, tm, tn, 0});
     taken.push_back({start, start + rows * cols});
     m.push_back(q);
   }
-  syms = product_tiles(m, true);
-  rects = product_tiles(m, false);
+  auto tasks = [&](const std::vector<Tile>& tiles) {
+    std::vector<Task> v;
+    for (const Tile& t : tiles) v.push_back({m[t.mat], t});
+    return v;
+  };
+  const std::vector<Task> packs = tasks(pack_tiles),
+                          syms = tasks(product_tiles(m, true)),
+                          rects = tasks(product_tiles(m, false));
   std::sort(taken.begin(), taken.end());
   int64_t at = 0;
   auto rest = [&](int64_t to) {
@@ -241,7 +252,7 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
       (int64_t)syms.size(), (int64_t)rects.size(), x_total, a_total};
   auto bytes = [](const auto& v) { return v.size() * sizeof(v[0]); };
   torch::Tensor tables = torch::empty(
-      {(int64_t)(bytes(m) + bytes(chunks) + bytes(packs) + bytes(syms)
+      {(int64_t)(bytes(chunks) + bytes(packs) + bytes(syms)
                  + bytes(rects))},
       torch::TensorOptions().dtype(torch::kUInt8));
   uint8_t* to = tables.data_ptr<uint8_t>();
@@ -249,7 +260,6 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
     if (!v.empty()) std::memcpy(to, v.data(), bytes(v));
     to += bytes(v);
   };
-  copy(m);
   copy(chunks);
   copy(packs);
   copy(syms);

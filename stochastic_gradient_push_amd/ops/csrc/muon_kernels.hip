@@ -64,6 +64,14 @@ static_assert(sizeof(Mat) == 64, "the host packs 64 bytes");
 // (big) of each.
 struct Tile { int mat, tm, tn, big; };
 
+// What a block has to do, in one piece: a record after another would be a
+// microsecond each at a kernel's start.
+struct Task {
+  Mat q;
+  Tile t;
+};
+static_assert(sizeof(Task) == 80, "the host packs 80 bytes");
+
 // Blocks go to the 8 XCDs in turn, each of which has an L2 of its own: the
 // `n` numbers are dealt so that an XCD gets neighbours.
 __device__ __forceinline__ int by_xcd(int block, int n) {
@@ -135,25 +143,26 @@ struct Uniform {
     if (k < down) return {id / strip, k, mt - 1, 0};
     return {id / strip, nt - 1, k - down, 0};
   }
-  __device__ Tile sym(int id) const { return tile(id, true, big_sym); }
-  __device__ Tile rect(int id) const { return tile(id, false, big_rect); }
-  __device__ Tile pack(int id) const {
+  __device__ Task task(Tile t) const { return {mat(t.mat), t}; }
+  __device__ Task sym(int id) const { return task(tile(id, true, big_sym)); }
+  __device__ Task rect(int id) const {
+    return task(tile(id, false, big_rect));
+  }
+  __device__ Task pack(int id) const {
     const int mt = first.mp / 64, per = first.np / 64 * mt, k = id % per;
-    return {id / per, k / mt, k % mt, 0};
+    return task({id / per, k / mt, k % mt, 0});
   }
   __device__ int chunk_mat(int id) const { return id / first.chunk1; }
 };
 
 // Matrices of any shapes: tables that the host has laid out.
 struct Table {
-  const Mat* mats;
-  const Tile* syms;
-  const Tile* rects;
-  const Tile* packs;
-  __device__ Mat mat(int i) const { return mats[i]; }
-  __device__ Tile sym(int id) const { return syms[id]; }
-  __device__ Tile rect(int id) const { return rects[id]; }
-  __device__ Tile pack(int id) const { return packs[id]; }
+  const Task* syms;
+  const Task* rects;
+  const Task* packs;
+  __device__ Task sym(int id) const { return syms[id]; }
+  __device__ Task rect(int id) const { return rects[id]; }
+  __device__ Task pack(int id) const { return packs[id]; }
 };
 
 // Sum over a block of 256 threads, the same in each; `lds` has 4 doubles.
@@ -329,8 +338,9 @@ __global__ __launch_bounds__(256) void k_ns_pack(
     float* __restrict__ r_out, float eps) {
   __shared__ double lds[4];
   __shared__ float tile[64][65];
-  const Tile t = src.pack(blockIdx.x);
-  const Mat q = src.mat(t.mat);
+  const Task task = src.pack(blockIdx.x);
+  const Tile t = task.t;
+  const Mat q = task.q;
   const bool tall = q.rows > q.cols;
   const int a0 = (tall ? t.tn : t.tm) * 64, b0 = (tall ? t.tm : t.tn) * 64;
   float v[2][8];
@@ -578,9 +588,11 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
   half_t* lds = reinterpret_cast<half_t*>(lds_raw);
   float* image = reinterpret_cast<float*>(lds_raw);
   constexpr bool LAST = MODE == APPLY && !__is_same(Out, ToPlanes);
-  const Tile t = MODE == APPLY ? src.rect(blockIdx.x) : src.sym(blockIdx.x);
+  const Task task = MODE == APPLY ? src.rect(blockIdx.x)
+                                  : src.sym(blockIdx.x);
+  const Tile t = task.t;
+  const Mat q = task.q;
   if (MODE != APPLY && t.tm > t.tn) return;  // below the diagonal
-  const Mat q = src.mat(t.mat);
   const int K = MODE == GRAM ? q.mp : q.np;
   const int q_rows = MODE == APPLY ? q.mp : q.np;
   const int64_t p_off = (MODE == GRAM ? q.x_off : q.a_off) + t.tm * 64 * 32;
@@ -1009,19 +1021,14 @@ void muon_step(float* p, const T* g, float* buf, __bf16* shadow,
                bool nesterov, int steps, Coef k, float eps,
                const void* tables, const int64_t* layout, void* work,
                double* partials, float* r, hipStream_t s) {
-  // layout: matrices, chunks, pack tiles, sym tiles, rect tiles, size of an
-  // X plane, size of an A plane; the tables lie in this order
+  // layout: matrices, chunks, tiles to pack, sym tiles, rect tiles, size of
+  // an X plane, size of an A plane; the tables lie in this order
   const char* at = static_cast<const char*>(tables);
-  Table src;
-  src.mats = reinterpret_cast<const Mat*>(at);
-  at += layout[0] * sizeof(Mat);
   const Chunk* chunks = reinterpret_cast<const Chunk*>(at);
-  at += layout[1] * sizeof(Chunk);
-  src.packs = reinterpret_cast<const Tile*>(at);
-  at += layout[2] * sizeof(Tile);
-  src.syms = reinterpret_cast<const Tile*>(at);
-  at += layout[3] * sizeof(Tile);
-  src.rects = reinterpret_cast<const Tile*>(at);
+  Table src;
+  src.packs = reinterpret_cast<const Task*>(chunks + layout[1]);
+  src.syms = src.packs + layout[2];
+  src.rects = src.syms + layout[3];
   if (layout[1] > 0)
     hipLaunchKernelGGL(k_muon_momentum<T>, dim3((unsigned)layout[1]),
                        dim3(256), 0, s, chunks, p, g, buf, shadow, lr, mu, wd,
