@@ -17,14 +17,14 @@ int sgp_ns_chunk();
 int64_t sgp_ns_big_tiles(int64_t tiles);
 bool sgp_ns_is_small(int n, int m);
 void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
-                       int batch, int steps, int split_steps, float a,
-                       float b, float c, float growth, float eps,
+                       int batch, int steps, int split_steps, int group,
+                       float a, float b, float c, float growth, float eps,
                        void* work, double* partials, float* r,
                        hipStream_t s);
 void sgp_muon_step(int dtype, float* p, const void* g, float* buf,
                    void* shadow, const float* lr, float mu, float wd,
-                   float rest_lr, bool nesterov, int steps, float a, float b,
-                   float c, float growth, float eps, const void* tables,
+                   float rest_lr, bool nesterov, int steps, int group, float a,
+                   float b, float c, float growth, float eps, const void* tables,
                    const int64_t* layout, void* work, double* partials,
                    float* r, hipStream_t s);
 }
@@ -73,9 +73,10 @@ Mat make_mat(int64_t start, int64_t rows, int64_t cols, double scale) {
   return q;
 }
 
-// fp16 values of workspace: X and its transpose twice, A and B, two planes
+// fp16 values of workspace: X and its transpose twice and five matrices of
+// A's size, two planes each
 int64_t work_size(int64_t x_total, int64_t a_total) {
-  return 8 * x_total + 4 * a_total;
+  return 8 * x_total + 10 * a_total;
 }
 
 int dtype_code(const torch::Tensor& t, const char* what) {
@@ -95,14 +96,15 @@ hipStream_t stream_of(const torch::Tensor& t) {
 
 // g: [batch, rows, cols]
 torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
-                            int64_t split_steps, double a, double b,
-                            double c, double growth, double eps) {
+                            int64_t split_steps, int64_t group, double a,
+                            double b, double c, double growth, double eps) {
   TORCH_CHECK(g.is_cuda() && g.is_contiguous() && g.dim() == 3,
               "newton_schulz: g must be a contiguous [batch, rows, cols] "
               "device tensor");
   const int dtype = dtype_code(g, "newton_schulz: g");
   TORCH_CHECK(steps >= 1 && steps <= 100 && split_steps >= 0
-              && split_steps <= steps, "newton_schulz: steps out of range");
+              && split_steps <= steps && group >= 1,
+              "newton_schulz: steps out of range");
   const c10::DeviceGuard guard(g.device());
   torch::Tensor out = torch::empty_like(g);
   if (g.numel() == 0) return out;
@@ -123,8 +125,8 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
     r = torch::empty({batch}, opt.dtype(torch::kFloat32));
   }
   sgp_newton_schulz(dtype, g.data_ptr(), out.data_ptr(), &q, (int)batch,
-                    (int)steps, (int)split_steps, (float)a, (float)b,
-                    (float)c, (float)growth, (float)eps,
+                    (int)steps, (int)split_steps, (int)group, (float)a,
+                    (float)b, (float)c, (float)growth, (float)eps,
                     work.defined() ? work.data_ptr() : nullptr,
                     work.defined() ? partials.data_ptr<double>() : nullptr,
                     work.defined() ? r.data_ptr<float>() : nullptr,
@@ -202,7 +204,7 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
   std::vector<Chunk> chunks;
   std::vector<Tile> pack_tiles;
   std::vector<std::pair<int64_t, int64_t>> taken;
-  int64_t x_total = 0, a_total = 0;
+  int64_t x_total = 0, a_total = 0, sum_nnm = 0, sum_nnn = 0;
   for (const auto& [start, rows, cols, scale] : mats) {
     TORCH_CHECK(start >= 0 && start + rows * cols <= total,
                 "muon: a matrix lies outside the flat buffer");
@@ -217,6 +219,8 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
                         (int)std::min<int64_t>(chunk, rows * cols - at), i});
     x_total += q.np * (int64_t)q.mp;
     a_total += q.np * (int64_t)q.np;
+    sum_nnm += (int64_t)q.np * q.np * q.mp;
+    sum_nnn += (int64_t)q.np * q.np * q.np;
     for (int tm = 0; tm < q.np / 64; ++tm)
       for (int tn = 0; tn < q.mp / 64; ++tn)
         pack_tiles.push_back({i, tm, tn, 0});
@@ -249,7 +253,8 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
 
   const std::vector<int64_t> layout = {
       (int64_t)m.size(), (int64_t)chunks.size(), (int64_t)packs.size(),
-      (int64_t)syms.size(), (int64_t)rects.size(), x_total, a_total};
+      (int64_t)syms.size(), (int64_t)rects.size(), x_total, a_total,
+      sum_nnm, sum_nnn};
   auto bytes = [](const auto& v) { return v.size() * sizeof(v[0]); };
   torch::Tensor tables = torch::empty(
       {(int64_t)(bytes(chunks) + bytes(packs) + bytes(syms)
@@ -281,8 +286,8 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
                 const torch::Tensor& tables,
                 const std::vector<int64_t>& layout, int64_t total,
                 const torch::Tensor& lr, double momentum, double weight_decay,
-                double rest_lr, bool nesterov, int64_t steps, double a,
-                double b, double c, double growth, double eps) {
+                double rest_lr, bool nesterov, int64_t steps, int64_t group,
+                double a, double b, double c, double growth, double eps) {
   check_flat(p, "params", p, torch::kFloat32);
   TORCH_CHECK(p.numel() == total, "muon_step_: the plan is for ", total,
               " values, params has ", p.numel());
@@ -300,8 +305,9 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
               "device");
   TORCH_CHECK(tables.device() == p.device(),
               "muon_step_: the plan is for another device");
-  TORCH_CHECK(layout.size() == 7, "muon_step_: not a plan");
-  TORCH_CHECK(steps >= 1 && steps <= 100, "muon_step_: steps out of range");
+  TORCH_CHECK(layout.size() == 9, "muon_step_: not a plan");
+  TORCH_CHECK(steps >= 1 && steps <= 100 && group >= 1,
+              "muon_step_: steps out of range");
   const c10::DeviceGuard guard(p.device());
   const auto opt = p.options();
   torch::Tensor work = torch::empty({work_size(layout[5], layout[6])},
@@ -313,8 +319,8 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
                 p.data_ptr<float>(), g.data_ptr(), buf.data_ptr<float>(),
                 shadow.has_value() ? shadow->data_ptr() : nullptr,
                 lr.data_ptr<float>(), (float)momentum, (float)weight_decay,
-                (float)rest_lr, nesterov, (int)steps, (float)a, (float)b,
-                (float)c, (float)growth, (float)eps, tables.data_ptr(),
+                (float)rest_lr, nesterov, (int)steps, (int)group, (float)a,
+                (float)b, (float)c, (float)growth, (float)eps, tables.data_ptr(),
                 layout.data(), work.data_ptr(), partials.data_ptr<double>(),
                 r.data_ptr<float>(), stream_of(p));
   C10_HIP_CHECK(hipGetLastError());

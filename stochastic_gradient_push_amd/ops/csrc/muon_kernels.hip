@@ -4,6 +4,18 @@
 //   X = G / (|G|_F + eps)                      [n, m], n <= m
 //   A = X X^T,  B = a I + b A + c A^2,  X = B X      (`steps` times)
 //
+// Steps in groups.  For wide matrices most of the work is in X X^T and B X,
+// while A, B and their products are n x n, symmetric, and commute.  So a
+// group of steps computes X X^T once and goes on with A alone,
+//
+//   B_k = a I + b A_k + c A_k^2,  A_{k+1} = B_k (B_k A_k),
+//   P_k = B_k P_{k-1},            X = P X   at the group's end.
+//
+// Two steps of m = 9 n take 3 n^2 m + 5 n^3 multiplications like this
+// instead of 6 n^2 m + 2 n^3 (symmetric results count half).  A's error grows with
+// the group, as that of a recomputed A does not: groups are of two steps
+// where the result is fp32 itself, of three elsewhere.
+//
 // All products run on the matrix cores, as row-by-row products C = P Q^T of
 // two operands whose rows lie along K: A = X X^T, A^2 = A A^T, and B X from
 // the transpose of X, which every step stores beside X.  A and A^2 are
@@ -384,7 +396,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(
 }
 
 // --------------------------------------------------------------- products
-enum { GRAM, POLY, APPLY };
+enum { GRAM, POLY, MUL, APPLY };
 
 struct Coef { float a, b, c, log2_growth; };
 
@@ -572,9 +584,11 @@ struct ToParams {
 };
 struct ToPlanes {};  // not the last product
 
-// C = P Q^T for one tile, and what its product makes of it:
+// C = P Q^T for one tile, and what its product makes of it in a group of
+// `group` steps that begins with step `step`:
 //   GRAM   A = X X^T            stored at its place and mirrored
 //   POLY   B = a I + b A + c A^2     likewise
+//   MUL    B M, symmetric       likewise
 //   APPLY  X = B X              stored, and transposed beside it; the last
 //                               one goes to `out`
 // Rounding, scaling and stores go through a 64-row image of the sums in LDS,
@@ -583,7 +597,7 @@ struct ToPlanes {};  // not the last product
 template <bool SPLIT, int MODE, class Src, class Out>
 __global__ __launch_bounds__(256, 2) void k_ns_gemm(
     Src src, Planes P, Planes Q, Planes C, Planes D, Out out,
-    const float* __restrict__ r, Coef k, int step) {
+    const float* __restrict__ r, Coef k, int step, int group) {
   __shared__ __attribute__((aligned(16))) char lds_raw[LDS_BYTES];
   half_t* lds = reinterpret_cast<half_t*>(lds_raw);
   float* image = reinterpret_cast<float*>(lds_raw);
@@ -596,13 +610,14 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
   const int K = MODE == GRAM ? q.mp : q.np;
   const int q_rows = MODE == APPLY ? q.mp : q.np;
   const int64_t p_off = (MODE == GRAM ? q.x_off : q.a_off) + t.tm * 64 * 32;
-  const int64_t q_off = (MODE == POLY ? q.a_off : q.x_off) + t.tn * 64 * 32;
+  const int64_t q_off = (MODE == POLY || MODE == MUL ? q.a_off : q.x_off)
+                        + t.tn * 64 * 32;
   const Operands o{{P.h + p_off, Q.h + q_off, SPLIT ? P.l + p_off : nullptr,
                     SPLIT ? Q.l + q_off : nullptr},
                    {(int64_t)q.np * 32, (int64_t)q_rows * 32}, K};
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
-  const float rr = MODE == POLY ? 0.f : r[t.mat];
+  const float rr = MODE == GRAM || MODE == APPLY ? r[t.mat] : 0.f;
 
   f32x4 acc[4][4];
 #pragma unroll
@@ -615,15 +630,15 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
     product64<SPLIT>(o, acc);
 
   // what the sums are multiplied with: powers of two, and r or its square
-  float f = 1.f / A_SCALE;
-  if (MODE != POLY) {
+  float f = MODE == MUL ? 1.f / B_SCALE : 1.f / A_SCALE;
+  if (MODE == GRAM || MODE == APPLY) {
     const int e = x_exp(q, rr, step, k);
     if (MODE == GRAM)
       f = ldexpf(rr * rr, -2 * e) * A_SCALE;
     else if (LAST)
       f = ldexpf(rr / B_SCALE, -e);
     else
-      f = ldexpf(1.f / B_SCALE, x_exp(q, rr, step + 1, k) - e);
+      f = ldexpf(1.f / B_SCALE, x_exp(q, rr, step + group, k) - e);
   }
 
   if (!t.big) {
@@ -907,10 +922,10 @@ __global__ __launch_bounds__(256) void k_ns_small(
   }
 }
 
-// Workspace, in fp16 values: X and its transpose twice, A and B, each as
-// two planes; x_total and a_total: the sizes of one plane.
+// Workspace, in fp16 values: X and its transpose twice, A, B A, B and P
+// twice, each as two planes; x_total and a_total: the sizes of one plane.
 struct Work {
-  Planes x[2], xt[2], a, b;
+  Planes x[2], xt[2], a, t, b, p[2];
 };
 
 Work split_work(void* base, int64_t x_total, int64_t a_total) {
@@ -924,48 +939,80 @@ Work split_work(void* base, int64_t x_total, int64_t a_total) {
   for (int i = 0; i < 2; ++i) {
     w.x[i] = take(x_total);
     w.xt[i] = take(x_total);
+    w.p[i] = take(a_total);
   }
   w.a = take(a_total);
+  w.t = take(a_total);
   w.b = take(a_total);
   return w;
 }
 
 Planes planes(Planes p, bool lo) { return {p.h, lo ? p.l : nullptr}; }
 
-template <bool SPLIT, int MODE, class Src, class Out>
-void product(Src src, Planes p, Planes q, Planes c, Planes d, Out out,
-             const float* r, Coef k, int step, int tiles, hipStream_t s) {
-  hipLaunchKernelGGL((k_ns_gemm<SPLIT, MODE, Src, Out>), dim3(tiles),
-                     dim3(256), 0, s, src, p, q, c, d, out, r, k, step);
-}
-
+// `count` steps, the first of them `step`, from X number `now` to the other,
+// or to `out`.
 template <bool SPLIT, class Src, class Out>
-void ns_step(Src src, const Work& w, int step, bool next_split, bool last,
-             Out out, const float* r, Coef k, int sym, int rect,
-             hipStream_t s) {
-  const int now = step & 1;
+void ns_group(Src src, const Work& w, int step, int count, int now,
+              bool next_split, bool last, Out out, const float* r, Coef k,
+              int n_sym, int n_rect, hipStream_t s) {
+  const dim3 block(256), sym(n_sym), rect(n_rect);
   const Planes x = w.x[now], xt = w.xt[now], none{nullptr, nullptr};
-  product<SPLIT, GRAM>(src, x, x, planes(w.a, SPLIT), none, ToPlanes{}, r, k,
-                       step, sym, s);
-  product<SPLIT, POLY>(src, w.a, w.a, planes(w.b, SPLIT), none, ToPlanes{},
-                       r, k, step, sym, s);
+  auto lo = [](Planes p) { return planes(p, SPLIT); };
+  auto mul = [&](Planes b, Planes m, Planes c) {
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, MUL, Src, ToPlanes>), sym, block, 0,
+                       s, src, b, m, lo(c), none, ToPlanes{}, r, k, step,
+                       count);
+  };
+  hipLaunchKernelGGL((k_ns_gemm<SPLIT, GRAM, Src, ToPlanes>), sym, block, 0,
+                     s, src, x, x, lo(w.a), none, ToPlanes{}, r, k, step,
+                     count);
+  for (int i = 0; i < count; ++i) {
+    // the first B is P itself
+    const Planes b = i == 0 ? w.p[0] : w.b;
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, POLY, Src, ToPlanes>), sym, block, 0,
+                       s, src, w.a, w.a, lo(b), none, ToPlanes{}, r, k, step,
+                       count);
+    if (i > 0) mul(b, w.p[(i - 1) & 1], w.p[i & 1]);
+    if (i + 1 < count) {
+      mul(b, w.a, w.t);
+      mul(b, w.t, w.a);
+    }
+  }
+  const Planes p = w.p[(count - 1) & 1];
   if (last)
-    product<SPLIT, APPLY>(src, w.b, xt, none, none, out, r, k, step, rect, s);
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, Out>), rect, block, 0, s,
+                       src, p, xt, none, none, out, r, k, step, count);
   else
-    product<SPLIT, APPLY>(src, w.b, xt, planes(w.x[now ^ 1], next_split),
-                          planes(w.xt[now ^ 1], next_split), ToPlanes{}, r,
-                          k, step, rect, s);
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, ToPlanes>), rect, block,
+                       0, s, src, p, xt, planes(w.x[now ^ 1], next_split),
+                       planes(w.xt[now ^ 1], next_split), ToPlanes{}, r, k,
+                       step, count);
 }
 
+// The first `split_steps` with pairs, in groups of up to `group`; the others
+// one by one.
 template <class Src, class Out>
-void ns_steps(Src src, const Work& w, int steps, int split_steps, Out out,
-              const float* r, Coef k, int sym, int rect, hipStream_t s) {
-  for (int i = 0; i < steps; ++i) {
-    auto f = i < split_steps ? ns_step<true, Src, Out>
-                             : ns_step<false, Src, Out>;
-    f(src, w, i, i + 1 < split_steps, i + 1 == steps, out, r, k, sym, rect,
-      s);
+void ns_steps(Src src, const Work& w, int steps, int split_steps, int group,
+              Out out, const float* r, Coef k, int n_sym, int n_rect,
+              hipStream_t s) {
+  int now = 0;
+  for (int i = 0; i < steps; now ^= 1) {
+    const bool split = i < split_steps;
+    const int left = split_steps - i;
+    const int count = !split ? 1 : left < group ? left : group;
+    auto f = split ? ns_group<true, Src, Out> : ns_group<false, Src, Out>;
+    f(src, w, i, count, now, i + count < split_steps, i + count == steps, out,
+      r, k, n_sym, n_rect, s);
+    i += count;
   }
+}
+
+// Steps of a group, of at most `most`, for matrices with sum_nnm = sum of
+// n^2 m and sum_nnn of n^3.  A further step in a group saves 3 n^2 m and costs
+// 3 n^3 and a launch (fp32, us, in groups and one by one: 512 x 1024 152 and
+// 147, 512 x 2048 166 and 173, 512 x 4608 226 and 267).
+int group_of(int most, double sum_nnm, double sum_nnn) {
+  return sum_nnm >= 3.0 * sum_nnn ? most : 1;
 }
 
 // Of `tiles` tiles of 128 x 128, how many to work on as such: two are on a
@@ -983,7 +1030,7 @@ bool is_small(int n, int m) { return n <= SMALL_N && m <= SMALL_M; }
 
 template <typename T>
 void newton_schulz(const T* g, T* out, const Mat& first, int batch, int steps,
-                   int split_steps, Coef k, float eps, void* work,
+                   int split_steps, int group, Coef k, float eps, void* work,
                    double* partials, float* r, hipStream_t s) {
   if (is_small(first.n, first.m)) {
     const Uniform src{first, batch, 0, 0};
@@ -1011,18 +1058,20 @@ void newton_schulz(const T* g, T* out, const Mat& first, int batch, int steps,
   const int64_t n_rect = big_rect + 4 * (rects - big_rect)
                          + batch * ((mt & 1 ? nt : 0)
                                     + (nt & 1 ? 2 * mb : 0));
-  ns_steps(src, w, steps, split_steps, ToTensor<T>{out}, r, k,
-           (int)n_sym, (int)n_rect, s);
+  const double n = first.np, m = first.mp;
+  ns_steps(src, w, steps, split_steps, group_of(group, n * n * m, n * n * n),
+           ToTensor<T>{out}, r, k, (int)n_sym, (int)n_rect, s);
 }
 
 template <typename T>
 void muon_step(float* p, const T* g, float* buf, __bf16* shadow,
                const float* lr, float mu, float wd, float rest_lr,
-               bool nesterov, int steps, Coef k, float eps,
+               bool nesterov, int steps, int group, Coef k, float eps,
                const void* tables, const int64_t* layout, void* work,
                double* partials, float* r, hipStream_t s) {
   // layout: matrices, chunks, tiles to pack, sym tiles, rect tiles, size of
-  // an X plane, size of an A plane; the tables lie in this order
+  // an X plane, size of an A plane, sums of n^2 m and of n^3; the tables lie
+  // in this order
   const char* at = static_cast<const char*>(tables);
   const Chunk* chunks = reinterpret_cast<const Chunk*>(at);
   Table src;
@@ -1039,8 +1088,10 @@ void muon_step(float* p, const T* g, float* buf, __bf16* shadow,
                      dim3((unsigned)layout[2]), dim3(256), 0, s, src,
                      Momentum<T>{g, buf, mu, nesterov}, partials, w.x[0],
                      w.xt[0], r, eps);
-  ns_steps(src, w, steps, steps, ToParams{p, shadow, lr, wd}, r, k,
-           (int)layout[3], (int)layout[4], s);
+  ns_steps(src, w, steps, steps,
+           group_of(group, (double)layout[7], (double)layout[8]),
+           ToParams{p, shadow, lr, wd}, r, k, (int)layout[3], (int)layout[4],
+           s);
 }
 
 }  // namespace
@@ -1056,7 +1107,7 @@ int64_t sgp_ns_big_tiles(int64_t tiles) { return big_tiles(tiles); }
 bool sgp_ns_is_small(int n, int m) { return is_small(n, m); }
 
 void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
-                       int batch, int steps, int split_steps,
+                       int batch, int steps, int split_steps, int group,
                        float a, float b, float c, float growth, float eps,
                        void* work, double* partials, float* r,
                        hipStream_t s) {
@@ -1064,32 +1115,32 @@ void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
   const Coef k{a, b, c, log2f(growth)};
   if (dtype == 0)
     newton_schulz(static_cast<const float*>(g), static_cast<float*>(out),
-                  first, batch, steps, split_steps, k, eps, work, partials, r,
-                  s);
+                  first, batch, steps, split_steps, group, k, eps, work,
+                  partials, r, s);
   else if (dtype == 1)
     newton_schulz(static_cast<const __bf16*>(g), static_cast<__bf16*>(out),
-                  first, batch, steps, split_steps, k, eps, work, partials, r,
-                  s);
+                  first, batch, steps, split_steps, group, k, eps, work,
+                  partials, r, s);
   else
     newton_schulz(static_cast<const half_t*>(g), static_cast<half_t*>(out),
-                  first, batch, steps, split_steps, k, eps, work, partials, r,
-                  s);
+                  first, batch, steps, split_steps, group, k, eps, work,
+                  partials, r, s);
 }
 
 void sgp_muon_step(int dtype, float* p, const void* g, float* buf,
                    void* shadow, const float* lr, float mu, float wd,
-                   float rest_lr, bool nesterov, int steps, float a, float b,
-                   float c, float growth, float eps, const void* tables,
+                   float rest_lr, bool nesterov, int steps, int group, float a,
+                   float b, float c, float growth, float eps, const void* tables,
                    const int64_t* layout, void* work, double* partials,
                    float* r, hipStream_t s) {
   const Coef k{a, b, c, log2f(growth)};
   __bf16* sh = static_cast<__bf16*>(shadow);
   if (dtype == 0)
     muon_step(p, static_cast<const float*>(g), buf, sh, lr, mu, wd, rest_lr,
-              nesterov, steps, k, eps, tables, layout, work, partials, r, s);
+              nesterov, steps, group, k, eps, tables, layout, work, partials, r, s);
   else
     muon_step(p, static_cast<const __bf16*>(g), buf, sh, lr, mu, wd, rest_lr,
-              nesterov, steps, k, eps, tables, layout, work, partials, r, s);
+              nesterov, steps, group, k, eps, tables, layout, work, partials, r, s);
 }
 
 }  // extern "C"

@@ -62,6 +62,16 @@ def _split_steps(steps: int, a: float, dtype: torch.dtype) -> int:
     return steps - single
 
 
+def _group(growth: float, most: int) -> int:
+    """How many steps may share one product with the whole matrix: up to
+    ``most``, while their common factor stays in the range that the kernels
+    hold such a matrix in."""
+    group = 1
+    while group < most and growth ** (group + 1) < 60.0:
+        group += 1
+    return group
+
+
 def _check_numbers(name, steps, coefficients, eps):
     if not isinstance(steps, int) or not 1 <= steps <= 100:
         raise ValueError(f"{name}: steps must be 1 to 100, got {steps}")
@@ -123,8 +133,9 @@ def newton_schulz(
     rows, cols = g.shape[-2:]
     out = _ext_for(g).newton_schulz(
         g.contiguous().view(g.shape[:-2].numel(), rows, cols), steps,
-        _split_steps(steps, coefficients[0], g.dtype), *coefficients, growth,
-        eps,
+        _split_steps(steps, coefficients[0], g.dtype),
+        _group(growth, 2 if g.dtype == torch.float32 else 3), *coefficients,
+        growth, eps,
     )
     return out.view(g.shape)
 
@@ -214,7 +225,7 @@ def muon_step_(
             params, grads, momentum_buf, shadow, plan.tables, plan.layout,
             plan.total, _as_scalar_tensor(lr, params), float(momentum),
             float(weight_decay), float(rest_lr), bool(nesterov), steps,
-            *coefficients, growth, eps,
+            _group(growth, 3), *coefficients, growth, eps,
         )
         return
     lr = float(lr)

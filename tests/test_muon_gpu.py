@@ -204,7 +204,7 @@ def test_refusals():
     with torch.no_grad():
         ops.newton_schulz(g.clone().requires_grad_(True))
     with pytest.raises(RuntimeError, match="contiguous"):
-        ext.newton_schulz(g, 5, 5, *COEF, 4.0, 1e-7)
+        ext.newton_schulz(g, 5, 5, 1, *COEF, 4.0, 1e-7)
     with pytest.raises(RuntimeError, match="2\\^20"):
         ops.newton_schulz(torch.empty(1, (1 << 20) + 1, device=dev()))
     plan = ops.MuonPlan([(0, 4, 6)], 24, "cuda")
@@ -296,7 +296,9 @@ def test_step_agrees_with_newton_schulz():
         part = slice(start, start + rows * cols)
         o = ops.newton_schulz(g[part].view(rows, cols)).reshape(-1)
         scale = max(1.0, rows / cols) ** 0.5
-        assert float((p[part] + scale * o).abs().max()) <= 1e-6 * scale
+        # the two may group their steps differently; each is within BOUND of
+        # the definition in the norm, so they are within twice that
+        assert float((p[part] + scale * o).norm()) <= 2 * BOUND * scale
 
 
 def test_optimizer_against_cpu():
