@@ -294,9 +294,13 @@ __global__ __launch_bounds__(256) void k_muon_momentum(
 }
 
 // ---------------------------------------------------------------- packing
-__device__ __forceinline__ half_t hi_of(float v) { return (half_t)v; }
-__device__ __forceinline__ half_t lo_of(float v, half_t hi) {
-  return (half_t)(v - (float)hi);
+// v = hi + lo.  v has to be settled as an fp32 number first: where it is a
+// product, the compiler may round that to fp16 for hi, and elsewhere to fp32
+// and then to fp16; if the two differ, lo belongs to the other.
+__device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
+  asm("" : "+v"(v));
+  hi = (half_t)v;
+  lo = (half_t)(v - (float)hi);
 }
 
 // What the matrices are read from: the first n <= 8 values from i on.
@@ -336,8 +340,10 @@ __device__ __forceinline__ void put8(const Planes& p, int64_t i,
   half8 h, l;
 #pragma unroll
   for (int x = 0; x < 8; ++x) {
-    h[x] = hi_of(v[x]);
-    l[x] = lo_of(v[x], h[x]);
+    half_t hi, lo;
+    split(v[x], hi, lo);
+    h[x] = hi;
+    l[x] = lo;
   }
   *reinterpret_cast<half8*>(p.h + i) = h;
   if (p.l != nullptr) *reinterpret_cast<half8*>(p.l + i) = l;
@@ -779,8 +785,10 @@ __device__ __forceinline__ void put4(half_t* h, int plane, const float* v) {
   half4 hi, lo;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    hi[x] = hi_of(v[x]);
-    lo[x] = lo_of(v[x], hi[x]);
+    half_t a, b;
+    split(v[x], a, b);
+    hi[x] = a;
+    lo[x] = b;
   }
   *reinterpret_cast<half4*>(h) = hi;
   *reinterpret_cast<half4*>(h + plane) = lo;
@@ -868,7 +876,8 @@ __global__ __launch_bounds__(256) void k_ns_small(
     for (int i = 0; i < 8; ++i) {
       if (first + i < total) {
         const float f = (float)((double)v[y][i] * inv);
-        const half_t h = hi_of(f), l = lo_of(f, h);
+        half_t h, l;
+        split(f, h, l);
         const int xr = tall ? col : row, xc = tall ? row : col;
         const int at = (int)place(xr, xc, SMALL_N), to = (int)place(xc, xr, MP);
         x[at] = h;
@@ -913,8 +922,7 @@ __global__ __launch_bounds__(256) void k_ns_small(
         half_t* to = x + place(r0, col, SMALL_N);  // a row: 8 further
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          to[i * 8] = hi_of(w[i]);
-          to[i * 8 + XP] = lo_of(w[i], hi_of(w[i]));
+          split(w[i], to[i * 8], to[i * 8 + XP]);
         }
       }
     }

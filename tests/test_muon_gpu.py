@@ -84,10 +84,12 @@ def test_shapes(shape, dtype):
         err, float(ref.norm()))
 
 
-@pytest.mark.parametrize("shape", [(64, 64), (200, 300), (128, 1152),
-                                   (512, 512), (700, 300)])
-def test_noise_against_fp32(shape):
-    g = torch.randn(*shape, device=dev())
+# at 1e-3 the norm is not so far above eps that |G| / (|G| + eps) is 1
+@pytest.mark.parametrize("scale", [1.0, 1e-3, 3e-6])
+@pytest.mark.parametrize("shape", [(64, 64), (64, 190), (200, 300),
+                                   (128, 1152), (512, 512), (700, 300)])
+def test_noise_against_fp32(shape, scale):
+    g = scale * torch.randn(*shape, device=dev())
     ref = factor(g)
     x = g.clone()
     tall = shape[0] > shape[1]
