@@ -11,10 +11,10 @@
 //   B_k = a I + b A_k + c A_k^2,  A_{k+1} = B_k (B_k A_k),
 //   P_k = B_k P_{k-1},            X = P X   at the group's end.
 //
-// Two steps of m = 9 n take 3 n^2 m + 5 n^3 multiplications like this
-// instead of 6 n^2 m + 2 n^3 (symmetric results count half).  A's error grows with
-// the group, as that of a recomputed A does not: groups are of two steps
-// where the result is fp32 itself, of three elsewhere.
+// Two steps take 3 n^2 m + 5 n^3 operations like this instead of 6 n^2 m +
+// 2 n^3 (symmetric results count half).  A's error grows within the group, as
+// that of a recomputed A does not: groups are of two steps where the result
+// is fp32 itself, of three elsewhere.
 //
 // All products run on the matrix cores, as row-by-row products C = P Q^T of
 // two operands whose rows lie along K: A = X X^T, A^2 = A A^T, and B X from
@@ -22,12 +22,19 @@
 // symmetric: only tiles on and above the diagonal are computed, and each
 // is stored twice.
 //
+// What bounds it.  4096 x 4096: a product of pairs runs at 1100 to 1200
+// TFLOP/s of fp16 work, as a large fp16 library product does; the matrix
+// pipes are busy 62% of the time at the 1.6 GHz that the power limit leaves.
+// Around 1000: the 64 x 64 tiles' loads from L2, 80 GB/s a CU.  Below 500:
+// the 17 launches, 4 us each.
+//
 // Precision.  A small singular value grows by the factor a in every step,
 // a^5 = 485 in all with the usual coefficients, and the rounding of X, A
 // and B grows with it.  Values are therefore held as two fp16 numbers,
 // v = hi + lo (22 bits), and a product is hi hi + hi lo + lo hi, three
-// matrix instructions with fp32 accumulation.  Where the result is 16 bits
-// wide anyway the last steps, whose roundings cannot grow any more, keep hi
+// matrix instructions with fp32 accumulation: errors are those of products
+// in fp32 or below (1000 x 2048: 1.0e-6 against 3.2e-6).  Where the result
+// is bf16 the last steps, whose roundings can hardly grow any more, keep hi
 // alone; the host says from which step on.
 //
 // Scales.  fp16 has a narrow range, so X is stored times 2^e, with e from
@@ -459,8 +466,8 @@ struct Fragments {
             o.at[2 * x + 1] + kt * o.next[1] + i * 512 + lane * 8);
       }
   }
-  // the three products of a pair one after another for all fragments: a
-  // matrix instruction that adds to the sum of the one before waits for it
+  // a pair's three products apart: a matrix instruction that adds to the sum
+  // of the one before it waits for that
   __device__ __forceinline__ void multiply(f32x4 (&acc)[F][F]) const {
 #pragma unroll
     for (int x = 0; x < (SPLIT ? 3 : 1); ++x)
@@ -484,8 +491,10 @@ __device__ __forceinline__ void arrive() {
 
 constexpr int LDS_BYTES = 65536;  // two blocks on a CU
 
-// 128 x 128, a wave 64 x 64 of it, 32 of K at a time.  K goes through S
-// buffers: while one is multiplied, the next S - 1 are on their way.
+// 128 x 128, a wave 64 x 64 of it, 32 of K at a time through S buffers.  While
+// one step is multiplied from registers, the next is read from LDS and those
+// behind it are on their way from memory.  Two blocks of 64 KB on a CU: one
+// of 128 KB with more buffers is 20% slower (all its waves wait at once).
 template <bool SPLIT>
 __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
                                            f32x4 (&acc)[4][4]) {
@@ -598,8 +607,8 @@ struct ToPlanes {};  // not the last product
 //   APPLY  X = B X              stored, and transposed beside it; the last
 //                               one goes to `out`
 // Rounding, scaling and stores go through a 64-row image of the sums in LDS,
-// from which 8 lanes read 64 neighbours of a row, or of a column: a stride
-// of an odd number of words keeps both free of conflicts.
+// from which 16 lanes read 8 columns of 16 rows, or 8 rows of 16 columns: with
+// an odd stride both ways two lanes meet at most.
 template <bool SPLIT, int MODE, class Src, class Out>
 __global__ __launch_bounds__(256, 2) void k_ns_gemm(
     Src src, Planes P, Planes Q, Planes C, Planes D, Out out,

@@ -218,6 +218,14 @@ def muon_step_(
             raise ValueError(f"muon_step_: {name} must have the plan's "
                              f"{plan.total} values, got shape "
                              f"{tuple(t.shape)}")
+    ends = sorted(
+        (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+        for t in (params, grads, momentum_buf, shadow)
+        if t is not None and t.numel()
+    )
+    if any(a[1] > b[0] for a, b in zip(ends, ends[1:])):
+        raise ValueError("muon_step_: params, grads, momentum_buf and shadow "
+                         "must not share memory")
     if params.is_cuda:
         from . import _as_scalar_tensor, _ext_for
 

@@ -313,6 +313,25 @@ def test_same_call_same_bits():
         assert all(torch.equal(first[k], again[k]) for k in first)
 
 
+def test_rows_beyond_32_bits():
+    rows, cols = (1 << 21) + 5, 1032
+    x = torch.zeros(rows, cols, device=dev(), dtype=torch.bfloat16)
+    assert x.numel() > 1 << 31
+    some, w, b, _, dy = inputs(4, cols, torch.bfloat16, torch.float32, False,
+                               False)
+    x[-4:] = some
+    leaf = x.requires_grad_(True)
+    g = torch.zeros_like(x)
+    g[-4:] = dy
+    y = ops.layer_norm(leaf, w, b)
+    dx, = torch.autograd.grad(y, leaf, g)
+    want = run(some, w, b, None, False, dy)
+    assert torch.equal(y[-4:], want["y"])
+    assert torch.equal(dx[-4:], want["dx"])
+    assert bool((dx[:-4] == 0).all())
+    assert torch.equal(y[0], b.to(torch.bfloat16))
+
+
 def test_no_rows():
     x = torch.empty(0, 64, device=dev(), requires_grad=True)
     w = torch.ones(64, device=dev(), requires_grad=True)

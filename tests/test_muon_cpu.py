@@ -113,6 +113,11 @@ def test_plan_refusals():
         ops.muon_step_(p[:9], p, p.clone(), plan, 0.1)
     with pytest.raises(ValueError, match="plan is for"):
         ops.muon_step_(p.to("meta"), p, p.clone(), plan, 0.1)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.muon_step_(p, torch.zeros(10), p, plan, 0.1)
+    both = torch.zeros(15)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.muon_step_(p, both[:10], both[5:], plan, 0.1)
 
 
 def step_oracle(p, g, buf, matrices, lr, mu, wd, nesterov, rest_lr):

@@ -117,7 +117,8 @@ def test_batches(batch, rows, cols):
     out = ops.newton_schulz(g)
     flat, each = g.view(-1, rows, cols), out.view(-1, rows, cols)
     for i in range(flat.shape[0]):
-        # a matrix's result does not depend on what lies beside it
+        # a matrix's result does not depend on what lies beside it (nor, at
+        # these sizes, on how many there are)
         assert torch.equal(each[i], ops.newton_schulz(flat[i])), i
 
 
@@ -175,11 +176,12 @@ def test_zeros_and_bad_values():
 
 
 @pytest.mark.parametrize("steps,coef", [
-    (1, COEF), (2, COEF), (10, COEF), (25, (1.5, -0.5, 0.0)),
+    (1, COEF), (2, COEF), (3, COEF), (4, COEF), (10, COEF), (25, (1.5, -0.5, 0.0)),
     (12, (1.875, -1.25, 0.375))])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_steps_and_coefficients(steps, coef, dtype):
-    g = torch.randn(90, 130, device=dev()).to(dtype)
+@pytest.mark.parametrize("cols", [130, 400])  # steps one by one, in groups
+def test_steps_and_coefficients(steps, coef, dtype, cols):
+    g = torch.randn(90, cols, device=dev()).to(dtype)
     ref = factor(g, steps, coef)
     out = ops.newton_schulz(g, steps=steps, coefficients=coef)
     # growth up to the result is at most that from the start to size 1: a
@@ -196,6 +198,38 @@ def test_same_call_same_bits():
     g = strong(300, 500, batch=(2,))
     first = ops.newton_schulz(g)
     assert all(torch.equal(ops.newton_schulz(g), first) for _ in range(3))
+
+
+@pytest.mark.parametrize("rows,cols,batch", [(64, 64, 530_000),
+                                             (256, 256, 33_000)])
+def test_batch_beyond_32_bits(rows, cols, batch):
+    g = torch.zeros(batch, rows, cols, device=dev(), dtype=torch.bfloat16)
+    assert g.numel() > 1 << 31
+    g[-2:] = strong(rows, cols, batch=(2,)).bfloat16()
+    out = ops.newton_schulz(g)
+    # against the definition, as in test_shapes: other tiles than for two
+    # matrices, so other last bits
+    for i in (-2, -1):
+        ref = factor(g[i])
+        err = float((out[i].double() - ref).norm())
+        assert err <= BOUND + rounding(ref, torch.bfloat16) \
+            + 6 * 12 * 2.0 ** -12 * float(ref.norm())
+    assert bool((out[:2] == 0).all()) and bool((out[-3] == 0).all())
+
+
+def test_step_beyond_32_bits():
+    total = (1 << 31) + 40_000
+    start = total - 20_001
+    plan = ops.MuonPlan([(start, 100, 200)], total, "cuda")
+    p, g, buf = (torch.zeros(total, device=dev()) for _ in range(3))
+    g[start:start + 20_000] = strong(100, 200).flatten()
+    g[-1] = 2.0
+    ops.muon_step_(p, g, buf, plan, 0.5, momentum=0.9, nesterov=False)
+    want = -0.5 * factor(g[start:start + 20_000].view(100, 200)).flatten()
+    got = p[start:start + 20_000].double()
+    assert float((got - want).norm()) <= 0.5 * BOUND
+    assert float(p[-1]) == -1.0 and float(buf[-1]) == 2.0
+    assert bool((p[:start] == 0).all())
 
 
 def test_refusals():
