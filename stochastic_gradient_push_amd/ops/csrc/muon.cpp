@@ -137,8 +137,9 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
 
 // The tiles of one product of all matrices: X X^T or A^2 (sym: on and above
 // the diagonal) or B X.  As many 128 x 128 tiles as fill the card, the
-// longest sums first, so that what starts last ends soon; of one matrix
-// the tiles that one XCD gets (every eighth block) are neighbours.
+// longest sums first, so that what starts last ends soon; of sums of one
+// length the tiles that one XCD gets (every eighth block) are neighbours: in
+// one matrix, or in few.
 std::vector<Tile> product_tiles(const std::vector<Mat>& m, bool sym) {
   auto length = [&](const Tile& t) { return sym ? m[t.mat].mp : m[t.mat].np; };
   auto longer = [&](const Tile& x, const Tile& y) {
@@ -178,7 +179,7 @@ std::vector<Tile> product_tiles(const std::vector<Mat>& m, bool sym) {
   big.insert(big.end(), small.begin(), small.end());
   for (size_t from = 0; from < big.size();) {
     size_t to = from;
-    while (to < big.size() && big[to].mat == big[from].mat
+    while (to < big.size() && length(big[to]) == length(big[from])
            && big[to].big == big[from].big)
       ++to;
     const std::vector<Tile> part(big.begin() + from, big.begin() + to);
