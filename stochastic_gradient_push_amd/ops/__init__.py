@@ -22,6 +22,9 @@ sgd_step_           fused momentum-SGD update (reference relies on
                                              torch.optim.SGD, ad_psgd.py:261-266)
 ==================  =====================================================
 
+Beside them, of their own modules: ``layer_norm`` (norm.py), and
+``newton_schulz``, ``MuonPlan`` and ``muon_step_`` (muon.py).
+
 Scalars ``a`` may be Python floats or 1-element device tensors (no host
 sync on the training path: push-sum weights stay device-resident).
 
