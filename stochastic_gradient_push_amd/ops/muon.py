@@ -48,17 +48,19 @@ def _growth(coefficients: Tuple[float, float, float], steps: int) -> float:
     return max(most, 1.0)
 
 
-def _split_steps(steps: int, a: float, dtype: torch.dtype) -> int:
+def _split_steps(steps: int, growth: float, dtype: torch.dtype) -> int:
     """How many steps need two fp16 numbers for a value.  A rounding to one
-    (2^-12) still grows by at most ``a`` in every step that follows, and in
-    its own.  While that is 16 in all it is no larger than the rounding of a
-    bf16 result (2^-9; measured 0.6 of it for noise, 0.95 for a few strong
-    directions).  fp16 and fp32 results need every step."""
+    (2^-11) grows by at most ``growth`` in its own step and in every one that
+    follows.  16 of them together, all at their largest, are twice the
+    rounding of a bf16 result (2^-8); in norm they stay below it (measured
+    0.6 of it for noise, 0.95 for a few strong directions).  fp16 and fp32
+    results need every step."""
     if dtype != torch.bfloat16:
         return steps
-    single = 0
-    while single < steps and a ** (single + 1) <= 16.0:
+    single, total = 0, growth
+    while single < steps and total <= 16.0:
         single += 1
+        total += growth ** (single + 1)
     return steps - single
 
 
@@ -133,7 +135,7 @@ def newton_schulz(
     rows, cols = g.shape[-2:]
     out = _ext_for(g).newton_schulz(
         g.contiguous().view(g.shape[:-2].numel(), rows, cols), steps,
-        _split_steps(steps, coefficients[0], g.dtype),
+        _split_steps(steps, growth, g.dtype),
         _group(growth, 2 if g.dtype == torch.float32 else 3), *coefficients,
         growth, eps,
     )

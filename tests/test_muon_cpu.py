@@ -96,6 +96,23 @@ def test_other_coefficients():
     assert float((sv - 1).abs().max()) < 1e-4
 
 
+@pytest.mark.parametrize("coef", [COEF, (1.5, -0.5, 0.0),
+                                  (1.875, -1.25, 0.375), (2.0, -1.5, 0.5)])
+@pytest.mark.parametrize("steps", [1, 2, 5, 10, 100])
+def test_steps_in_one_number(coef, steps):
+    """As many last steps as let their roundings grow to 16 in all."""
+    from stochastic_gradient_push_amd.ops import muon
+
+    growth = muon._growth(coef, steps)
+    for dtype in (torch.float32, torch.float16):
+        assert muon._split_steps(steps, growth, dtype) == steps
+    single = steps - muon._split_steps(steps, growth, torch.bfloat16)
+    assert 0 <= single <= steps
+    assert sum(growth ** k for k in range(1, single + 1)) <= 16
+    assert single == steps or sum(
+        growth ** k for k in range(1, single + 2)) > 16
+
+
 def test_plan_refusals():
     with pytest.raises(ValueError, match="overlaps"):
         ops.MuonPlan([(0, 2, 3), (5, 1, 1)], 10, "cpu")

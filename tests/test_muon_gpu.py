@@ -10,6 +10,8 @@ where the input is noise: at most four times the error of the same formulas
 in fp32, two bits for 22-bit values instead of 24.
 """
 
+import copy
+
 import pytest
 import torch
 
@@ -194,6 +196,19 @@ def test_steps_and_coefficients(steps, coef, dtype, cols):
     assert err <= bound + rounding(ref, dtype) + single
 
 
+@pytest.mark.parametrize("steps,coef", [
+    (8, (1.5, -0.5, 0.0)), (6, (1.875, -1.25, 0.375)), (8, (2.0, -1.5, 0.5))])
+@pytest.mark.parametrize("shape", [(64, 100), (90, 400), (300, 200)])
+def test_bf16_with_slow_coefficients(steps, coef, shape):
+    # the steps in 11 bits add what 16 roundings of 2^-11 do if all of them
+    # are the largest, twice the 2^-8 of the result's own; noise, half of it
+    g = torch.randn(*shape, device=dev()).bfloat16()
+    ref = factor(g, steps, coef)
+    own = float((ref.bfloat16().double() - ref).norm())
+    out = ops.newton_schulz(g, steps=steps, coefficients=coef)
+    assert float((out.double() - ref).norm()) <= 2 * own
+
+
 def test_same_call_same_bits():
     g = strong(300, 500, batch=(2,))
     first = ops.newton_schulz(g)
@@ -356,6 +371,33 @@ def test_optimizer_against_cpu():
         # each within BOUND times lr of the definition, and so is the CPU
         assert float((opts[0].flatp.flat - opts[1].flatp.flat.cpu())
                      .abs().max()) <= 3 * 2 * 0.1 * BOUND
+
+
+def test_working_weights_and_sgd_params():
+    """bf16 working weights with a matrix among the SGD parameters: the
+    cast section has matrices and plain values, the rest none."""
+    torch.manual_seed(2)
+    nets = [resnet18(num_classes=10, norm="layer")]
+    nets.append(copy.deepcopy(nets[0]).to(dev()))
+    opts = []
+    for net in nets:
+        gdp = GossipDataParallel(net, rank=0, world_size=1,
+                                 working_dtype=torch.bfloat16)
+        opts.append(FusedMuon(
+            gdp.flatp, lr=0.1, weight_decay=0.01, rest_lr=0.5,
+            sgd_params=[net.fc.weight, net.conv1.weight], steal_grads=True))
+    for _ in range(2):
+        for p, q in zip(nets[0].parameters(), nets[1].parameters()):
+            p.grad = torch.randn_like(p)
+            q.grad = p.grad.to(dev())
+        for opt in opts:
+            opt.step()
+    flat = opts[1].flatp
+    # in two steps each matrix stays within BOUND times lr and its scale (at
+    # most sqrt(2): the downsampling ones) of the definition, and so the CPU
+    assert float((opts[0].flatp.flat - flat.flat.cpu()).abs().max()) <= (
+        2 * 2 * 0.1 * 2 ** 0.5 * BOUND)
+    assert torch.equal(flat.shadow, flat.flat[:flat.n_cast].bfloat16())
 
 
 def _training(steps, capture):
