@@ -1026,10 +1026,16 @@ void ns_steps(Src src, const Work& w, int steps, int split_steps, int group,
 
 // Steps of a group, of at most `most`, for matrices with sum_nnm = sum of
 // n^2 m and sum_nnn of n^3.  A further step in a group saves 3 n^2 m and costs
-// 3 n^3 and a launch (fp32, us, in groups and one by one: 512 x 1024 152 and
-// 147, 512 x 2048 166 and 173, 512 x 4608 226 and 267).
+// 3 n^3, in products that fill the card less well, and a launch.  One by one
+// and in groups, fp32, us:
+//   128 x 1152 112, 110   256 x 512 110, 118   256 x 2304 163, 150
+//   512 x 1024 148, 156   512 x 2048 175, 170   1000 x 2048 237, 235
+//   1024 x 1536 218, 223   2048 x 2560 772, 781   2048 x 4096 1022, 944
+//   4 of 512 x 1024 173, 169   4096 x 8192 6036, 5140
+// so from m = 3 n on, and from m = 2 n on where the difference is large.
 int group_of(int most, double sum_nnm, double sum_nnn) {
-  return sum_nnm >= 3.0 * sum_nnn ? most : 1;
+  const double more = sum_nnm - sum_nnn;
+  return more >= 2.0 * sum_nnn || (more >= sum_nnn && more >= 4e8) ? most : 1;
 }
 
 // Of `tiles` tiles of 128 x 128, how many to work on as such: two are on a

@@ -112,6 +112,24 @@ def test_noise_against_fp32(shape, scale):
     assert err <= 2 * own, (err, own)
 
 
+def test_noise_in_groups_of_large_matrices():
+    # steps in groups from m = 2 n on, at four times the error of the same
+    # formulas in fp32 like smaller ones
+    g = torch.randn(800, 1700, device=dev())
+    ref = factor(g)
+    x = g / (g.norm() + 1e-7)
+    a, b, c = COEF
+    for _ in range(5):
+        s = x @ x.T
+        x = a * x + (b * s + c * (s @ s)) @ x
+    plain = float((x.double() - ref).norm())
+    for h in (g, g.T):
+        out = ops.newton_schulz(h)
+        out = out if h is g else out.T
+        err = float((out.double() - ref).norm())
+        assert err <= 4 * plain + 4 * 2.0 ** -24 * float(ref.norm())
+
+
 @pytest.mark.parametrize("batch,rows,cols", [
     ((5,), 48, 80), ((2, 3), 100, 70), ((3,), 300, 270), ((17,), 16, 5)])
 def test_batches(batch, rows, cols):
