@@ -26,7 +26,7 @@
 // TFLOP/s of fp16 work, as a large fp16 library product does; the matrix
 // pipes are busy 62% of the time at the 1.6 GHz that the power limit leaves.
 // Around 1000: the 64 x 64 tiles' loads from L2, 80 GB/s a CU.  Below 500:
-// the 17 launches, 4 us each.
+// the 17 to 21 launches, 4 us each.
 //
 // Precision.  A small singular value grows by the factor a in every step,
 // a^5 = 485 in all with the usual coefficients, and the rounding of X, A
@@ -603,7 +603,7 @@ struct ToPlanes {};  // not the last product
 // `group` steps that begins with step `step`:
 //   GRAM   A = X X^T            stored at its place and mirrored
 //   POLY   B = a I + b A + c A^2     likewise
-//   MUL    B M, symmetric       likewise
+//   MUL    B M, symmetric       likewise; the grid's second row: B M2 to D
 //   APPLY  X = B X              stored, and transposed beside it; the last
 //                               one goes to `out`
 // Rounding, scaling and stores go through a 64-row image of the sums in LDS,
@@ -611,8 +611,12 @@ struct ToPlanes {};  // not the last product
 // an odd stride both ways two lanes meet at most.
 template <bool SPLIT, int MODE, class Src, class Out>
 __global__ __launch_bounds__(256, 2) void k_ns_gemm(
-    Src src, Planes P, Planes Q, Planes C, Planes D, Out out,
+    Src src, Planes P, Planes Q, Planes Q2, Planes C, Planes D, Out out,
     const float* __restrict__ r, Coef k, int step, int group) {
+  if (MODE == MUL && blockIdx.y == 1) {
+    Q = Q2;
+    C = D;
+  }
   __shared__ __attribute__((aligned(16))) char lds_raw[LDS_BYTES];
   half_t* lds = reinterpret_cast<half_t*>(lds_raw);
   float* image = reinterpret_cast<float*>(lds_raw);
@@ -975,33 +979,38 @@ void ns_group(Src src, const Work& w, int step, int count, int now,
   const dim3 block(256), sym(n_sym), rect(n_rect);
   const Planes x = w.x[now], xt = w.xt[now], none{nullptr, nullptr};
   auto lo = [](Planes p) { return planes(p, SPLIT); };
-  auto mul = [&](Planes b, Planes m, Planes c) {
-    hipLaunchKernelGGL((k_ns_gemm<SPLIT, MUL, Src, ToPlanes>), sym, block, 0,
-                       s, src, b, m, lo(c), none, ToPlanes{}, r, k, step,
-                       count);
+  // c = b m, and in the same launch d = b m2 where there is one (a step over
+  // ResNet-18's matrices 356 -> 343 us, over ResNet-50's 793 -> 762)
+  auto mul = [&](Planes b, Planes m, Planes c, Planes m2, Planes d) {
+    hipLaunchKernelGGL((k_ns_gemm<SPLIT, MUL, Src, ToPlanes>),
+                       dim3(n_sym, m2.h != nullptr ? 2 : 1), block, 0, s, src,
+                       b, m, m2, lo(c), lo(d), ToPlanes{}, r, k, step, count);
   };
   hipLaunchKernelGGL((k_ns_gemm<SPLIT, GRAM, Src, ToPlanes>), sym, block, 0,
-                     s, src, x, x, lo(w.a), none, ToPlanes{}, r, k, step,
-                     count);
+                     s, src, x, x, none, lo(w.a), none, ToPlanes{}, r, k,
+                     step, count);
   for (int i = 0; i < count; ++i) {
     // the first B is P itself
     const Planes b = i == 0 ? w.p[0] : w.b;
+    const Planes before = i == 0 ? none : w.p[(i - 1) & 1];
     hipLaunchKernelGGL((k_ns_gemm<SPLIT, POLY, Src, ToPlanes>), sym, block, 0,
-                       s, src, w.a, w.a, lo(b), none, ToPlanes{}, r, k, step,
-                       count);
-    if (i > 0) mul(b, w.p[(i - 1) & 1], w.p[i & 1]);
+                       s, src, w.a, w.a, none, lo(b), none, ToPlanes{}, r, k,
+                       step, count);
     if (i + 1 < count) {
-      mul(b, w.a, w.t);
-      mul(b, w.t, w.a);
+      mul(b, w.a, w.t, before, w.p[i & 1]);
+      mul(b, w.t, w.a, none, none);
+    } else if (i > 0) {
+      mul(b, before, w.p[i & 1], none, none);
     }
   }
   const Planes p = w.p[(count - 1) & 1];
   if (last)
     hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, Out>), rect, block, 0, s,
-                       src, p, xt, none, none, out, r, k, step, count);
+                       src, p, xt, none, none, none, out, r, k, step, count);
   else
     hipLaunchKernelGGL((k_ns_gemm<SPLIT, APPLY, Src, ToPlanes>), rect, block,
-                       0, s, src, p, xt, planes(w.x[now ^ 1], next_split),
+                       0, s, src, p, xt, none,
+                       planes(w.x[now ^ 1], next_split),
                        planes(w.xt[now ^ 1], next_split), ToPlanes{}, r, k,
                        step, count);
 }
