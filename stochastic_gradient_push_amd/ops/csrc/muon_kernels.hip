@@ -554,23 +554,37 @@ __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
 // 1 KB of contiguous memory, so it comes straight into registers; nothing is
 // shared between the waves before the end, and LDS, which would be the
 // bottleneck, stays out of it.  The next step's loads are on their way while
-// one is multiplied.
+// one is multiplied; none of them depends on a condition inside the loop, so
+// that the waits count exactly what was issued since.
 template <bool SPLIT>
 __device__ __forceinline__ void product64(const Operands& o,
                                           f32x4 (&acc)[4][4]) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int KT = o.K / 32;
+  const int steps = (o.K / 32 - wave + 3) / 4;  // wave, wave + 4, ...
   Fragments<SPLIT, 4> f[2];
-  if (wave < KT) f[0].load(o, wave, lane);
-  for (int kt = wave; kt < KT; kt += 8) {
-    if (kt + 4 < KT) f[1].load(o, kt + 4, lane);
-    f[0].multiply(acc);
-    if (kt + 4 < KT) {
-      if (kt + 8 < KT) f[0].load(o, kt + 8, lane);
+  auto load = [&](int x, int step) {
+    __builtin_amdgcn_sched_barrier(0);
+    f[x].load(o, wave + 4 * step, lane);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (steps < 1) return;
+  load(0, 0);
+  if (steps > 1) {
+    load(1, 1);
+    int i = 2;  // the next to load
+    for (; i + 1 < steps; i += 2) {
+      f[0].multiply(acc);
+      load(0, i);
       f[1].multiply(acc);
+      load(1, i + 1);
     }
+    f[0].multiply(acc);
+    if (i < steps) load(0, i);
+    f[1].multiply(acc);
+    if (i == steps) return;
   }
+  f[0].multiply(acc);
 }
 
 // Where the last product goes, the first n <= 8 values from i on: a tensor,
