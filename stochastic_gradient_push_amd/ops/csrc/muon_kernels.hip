@@ -455,29 +455,48 @@ struct Fragments {
             lds + (2 * x + 1) * plane + (q_row + i * 16) * 32 + lane * 8);
       }
   }
-  __device__ __forceinline__ void load(const Operands& o, int kt, int lane) {
-#pragma unroll
-    for (int x = 0; x < NP; ++x)
+  // fragment i of plane x, as in Operands
+  __device__ __forceinline__ void load(const Operands& o, int kt, int lane,
+                                       int x, int i) {
+    half8& to = (x & 1 ? b : a)[x >> 1][i];
+    to = *reinterpret_cast<const half8*>(
+        o.at[x] + kt * o.next[x & 1] + i * 512 + lane * 8);
+  }
+  // A pair's three products apart: a matrix instruction that adds to the sum
+  // of the one before it waits for that.  done(x, i): fragment i of plane x
+  // is not needed any more.
+  template <class Done>
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[F][F],
+                                           Done done) const {
+    auto mul = [&](int x, int y, int i, int j) {
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[x][i], b[y][j],
+                                                         acc[i][j], 0, 0, 0);
+    };
+    if constexpr (SPLIT) {
 #pragma unroll
       for (int i = 0; i < F; ++i) {
-        a[x][i] = *reinterpret_cast<const half8*>(
-            o.at[2 * x] + kt * o.next[0] + i * 512 + lane * 8);
-        b[x][i] = *reinterpret_cast<const half8*>(
-            o.at[2 * x + 1] + kt * o.next[1] + i * 512 + lane * 8);
+#pragma unroll
+        for (int j = 0; j < F; ++j) mul(1, 0, i, j);
+        done(2, i);
       }
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+#pragma unroll
+        for (int i = 0; i < F; ++i) mul(0, 0, i, j);
+        done(1, j);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+#pragma unroll
+      for (int j = 0; j < F; ++j) mul(0, NP - 1, i, j);
+      done(0, i);
+    }
+#pragma unroll
+    for (int j = 0; j < F; ++j) done(2 * NP - 1, j);
   }
-  // a pair's three products apart: a matrix instruction that adds to the sum
-  // of the one before it waits for that
   __device__ __forceinline__ void multiply(f32x4 (&acc)[F][F]) const {
-#pragma unroll
-    for (int x = 0; x < (SPLIT ? 3 : 1); ++x)
-#pragma unroll
-      for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              a[x == 2 ? NP - 1 : 0][i], b[x == 1 ? NP - 1 : 0][j],
-              acc[i][j], 0, 0, 0);
+    multiply(acc, [](int, int) {});
   }
 };
 
@@ -554,8 +573,10 @@ __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
 // 1 KB of contiguous memory, so it comes straight into registers; nothing is
 // shared between the waves before the end, and LDS, which would be the
 // bottleneck, stays out of it.  The next step's loads are on their way while
-// one is multiplied; none of them depends on a condition inside the loop, so
-// that the waits count exactly what was issued since.
+// one is multiplied.  The four waves' loads take longer to issue than their
+// products, so a fragment is loaded anew as soon as it is not needed any
+// more, between the products.  No load depends on a condition inside the
+// loop, so that a wait counts exactly what was issued since.
 template <bool SPLIT>
 __device__ __forceinline__ void product64(const Operands& o,
                                           f32x4 (&acc)[4][4]) {
@@ -563,24 +584,32 @@ __device__ __forceinline__ void product64(const Operands& o,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int steps = (o.K / 32 - wave + 3) / 4;  // wave, wave + 4, ...
   Fragments<SPLIT, 4> f[2];
-  auto load = [&](int x, int step) {
-    __builtin_amdgcn_sched_barrier(0);
-    f[x].load(o, wave + 4 * step, lane);
-    __builtin_amdgcn_sched_barrier(0);
+  // in the order of their use
+  auto load = [&](Fragments<SPLIT, 4>& to, int step) {
+#pragma unroll
+    for (int x : {2, 1, 0, 3})
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (SPLIT || x < 2) to.load(o, wave + 4 * step, lane, x, i);
+  };
+  auto turn = [&](Fragments<SPLIT, 4>& g, int step) {
+    g.multiply(acc, [&](int x, int i) {
+      __builtin_amdgcn_sched_barrier(0);
+      g.load(o, wave + 4 * step, lane, x, i);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
   if (steps < 1) return;
-  load(0, 0);
+  load(f[0], 0);
   if (steps > 1) {
-    load(1, 1);
+    load(f[1], 1);
     int i = 2;  // the next to load
     for (; i + 1 < steps; i += 2) {
-      f[0].multiply(acc);
-      load(0, i);
-      f[1].multiply(acc);
-      load(1, i + 1);
+      turn(f[0], i);
+      turn(f[1], i + 1);
     }
     f[0].multiply(acc);
-    if (i < steps) load(0, i);
+    if (i < steps) load(f[0], i);
     f[1].multiply(acc);
     if (i == steps) return;
   }
