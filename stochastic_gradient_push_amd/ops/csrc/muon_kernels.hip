@@ -443,19 +443,13 @@ template <bool SPLIT, int F>
 struct Fragments {
   static constexpr int NP = SPLIT ? 2 : 1;
   half8 a[NP][F], b[NP][F];
-  __device__ __forceinline__ void read(const half_t* lds, int plane,
-                                       int p_row, int q_row, int lane) {
-#pragma unroll
-    for (int x = 0; x < NP; ++x)
-#pragma unroll
-      for (int i = 0; i < F; ++i) {
-        a[x][i] = *reinterpret_cast<const half8*>(
-            lds + 2 * x * plane + (p_row + i * 16) * 32 + lane * 8);
-        b[x][i] = *reinterpret_cast<const half8*>(
-            lds + (2 * x + 1) * plane + (q_row + i * 16) * 32 + lane * 8);
-      }
+  // fragment i of plane x, as in Operands, at `row` of that plane in LDS
+  __device__ __forceinline__ void read(const half_t* plane, int row, int lane,
+                                       int x, int i) {
+    (x & 1 ? b : a)[x >> 1][i] =
+        *reinterpret_cast<const half8*>(plane + row * 32 + lane * 8);
   }
-  // fragment i of plane x, as in Operands
+  // the same from memory
   __device__ __forceinline__ void load(const Operands& o, int kt, int lane,
                                        int x, int i) {
     half8& to = (x & 1 ? b : a)[x >> 1][i];
@@ -501,41 +495,73 @@ struct Fragments {
 };
 
 // Everything but the newest N direct loads has arrived, for every wave, and
-// every wave is done with what it read before.
+// every wave is done with what it read before.  The compiler knows of this
+// wait, and adds none of its own for what was read before it.
 template <int N>
 __device__ __forceinline__ void arrive() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N)
-               : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 constexpr int LDS_BYTES = 65536;  // two blocks on a CU
 
 // 128 x 128, a wave 64 x 64 of it, 32 of K at a time through S buffers.  While
 // one step is multiplied from registers, the next is read from LDS and those
-// behind it are on their way from memory.  Two blocks of 64 KB on a CU: one
-// of 128 KB with more buffers is 20% slower (all its waves wait at once).
+// behind it are on their way from memory; reads and loads are issued between
+// the products, which they would hold up in one piece (a pair's B X at 4096 x
+// 4096, before the power limit slows it: 325 us instead of 341).  Two blocks
+// of 64 KB on a CU: one of 128 KB with more buffers is 20% slower (all its
+// waves wait at once).
 template <bool SPLIT>
 __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
                                            f32x4 (&acc)[4][4]) {
   constexpr int NP = SPLIT ? 2 : 1, PLANE = 128 * 32;
   constexpr int S = LDS_BYTES / (2 * NP * PLANE * 2);
-  constexpr int L = 4 * NP;         // direct loads of a wave for 32 of K
+  constexpr int L = 4 * NP;  // direct loads of a wave for 32 of K
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto fetch_one = [&](int kt, int buf, int x, int i) {
+    load_lds(o.at[x] + kt * o.next[x & 1] + (i * 4 + wave) * 512 + lane * 8,
+             lds + (buf * 2 * NP + x) * PLANE + (i * 4 + wave) * 512);
+  };
   auto fetch = [&](int kt, int buf) {
 #pragma unroll
     for (int x = 0; x < 2 * NP; ++x)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        load_lds(o.at[x] + kt * o.next[x & 1] + (i * 4 + wave) * 512
-                     + lane * 8,
-                 lds + (buf * 2 * NP + x) * PLANE + (i * 4 + wave) * 512);
+      for (int i = 0; i < 2; ++i) fetch_one(kt, buf, x, i);
+  };
+  auto read_one = [&](Fragments<SPLIT, 4>& f, int buf, int x, int i) {
+    f.read(lds + (buf * 2 * NP + x) * PLANE,
+           ((x & 1 ? wave & 1 : wave >> 1) * 4 + i) * 16, lane, x, i);
   };
   auto read = [&](Fragments<SPLIT, 4>& f, int buf) {
-    f.read(lds + buf * 2 * NP * PLANE, PLANE, (wave >> 1) * 64,
-           (wave & 1) * 64, lane);
+#pragma unroll
+    for (int x = 0; x < 2 * NP; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) read_one(f, buf, x, i);
   };
-  const int KT = o.K / 32;  // even
+  // multiplies f, and between the products reads `next` from its buffer and
+  // fetches step kt to the one that f came from
+  auto turn = [&](Fragments<SPLIT, 4>& f, Fragments<SPLIT, 4>& next, int from,
+                  int kt, int to) {
+    int n = 0;
+    f.multiply(acc, [&](int, int) {
+      if (n < 4 * NP) {
+        __builtin_amdgcn_sched_barrier(0);
+        read_one(next, from, n >> 1, (2 * n) & 3);
+        read_one(next, from, n >> 1, (2 * n + 1) & 3);
+        fetch_one(kt, to, n >> 1, n & 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      ++n;
+    });
+  };
+  const int KT = o.K / 32;  // even, like S
 #pragma unroll
   for (int kt = 0; kt < S; ++kt)
     if (kt < KT) fetch(kt, kt);
@@ -545,25 +571,24 @@ __device__ __forceinline__ void product128(const Operands& o, half_t* lds,
   else
     arrive<0>();
   read(f[0], 0);
-  int buf = 0;  // of f[0]
-  for (int kt = 0; kt < KT; kt += 2) {
-    // f[0] has kt; kt + 1 is read and kt + S fetched while it is multiplied
-    if (kt + S <= KT)
-      arrive<(S - 2) * L>();
-    else
-      arrive<0>();
-    const int b1 = buf + 1 == S ? 0 : buf + 1;
-    read(f[1], b1);
-    if (kt + S < KT) fetch(kt + S, buf);
+  int buf = 0, kt = 0;  // f[0] has kt, and buf is where it was read from
+  auto after = [&](int b) { return b + 1 == S ? 0 : b + 1; };
+  for (; kt + S < KT; kt += 2) {
+    arrive<(S - 2) * L>();
+    const int b1 = after(buf);
+    turn(f[0], f[1], b1, kt + S, buf);
+    arrive<(S - 2) * L>();
+    buf = after(b1);
+    turn(f[1], f[0], buf, kt + 1 + S, b1);
+  }
+  arrive<0>();
+  for (; kt < KT; kt += 2) {  // nothing left to fetch
+    buf = after(buf);
+    read(f[1], buf);
     f[0].multiply(acc);
-    buf = b1 + 1 == S ? 0 : b1 + 1;
     if (kt + 2 < KT) {
-      if (kt + 1 + S <= KT)
-        arrive<(S - 2) * L>();
-      else
-        arrive<0>();
+      buf = after(buf);
       read(f[0], buf);
-      if (kt + 1 + S < KT) fetch(kt + 1 + S, b1);
     }
     f[1].multiply(acc);
   }
