@@ -24,9 +24,10 @@
 //
 // What bounds it.  4096 x 4096: a product of pairs runs at 1100 to 1200
 // TFLOP/s of fp16 work, as a large fp16 library product does; the matrix
-// pipes are busy 62% of the time at the 1.6 GHz that the power limit leaves.
-// Around 1000: the 64 x 64 tiles' loads from L2, 80 GB/s a CU.  Below 500:
-// the 17 to 21 launches, 4 us each.
+// pipes are busy 67% of the time at the 1.6 GHz that the power limit leaves.
+// Around 1000: the 64 x 64 tiles' loads, 95 GB/s a CU (nothing but loads: 145
+// from L2, 90 to 120 from behind it).  Below 500: the 17 to 21 launches, 4 us
+// each.
 //
 // Precision.  A small singular value grows by the factor a in every step,
 // a^5 = 485 in all with the usual coefficients, and the rounding of X, A
