@@ -14,7 +14,7 @@
 
 extern "C" {
 int sgp_ns_chunk();
-int64_t sgp_ns_big_tiles(int64_t tiles);
+int64_t sgp_ns_plan_big_tiles(int64_t tiles, bool sym);
 bool sgp_ns_is_small(int n, int m);
 void sgp_newton_schulz(int dtype, const void* g, void* out, const void* mat,
                        int batch, int steps, int split_steps, int group,
@@ -165,7 +165,8 @@ std::vector<Tile> product_tiles(const std::vector<Mat>& m, bool sym) {
         }
   }
   std::stable_sort(big.begin(), big.end(), longer);
-  const size_t keep = (size_t)sgp_ns_big_tiles((int64_t)big.size());
+  const size_t keep =
+      (size_t)sgp_ns_plan_big_tiles((int64_t)big.size(), sym);
   for (size_t i = keep; i < big.size(); ++i)
     for (int k = 0; k < 4; ++k) {
       const Tile t{big[i].mat, big[i].tm + (k & 1), big[i].tn + (k >> 1), 0};

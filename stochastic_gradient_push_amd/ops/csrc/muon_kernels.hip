@@ -1116,14 +1116,24 @@ int group_of(int most, double sum_nnm, double sum_nnn) {
   return more >= 2.0 * sum_nnn || (more >= sum_nnn && more >= 4e8) ? most : 1;
 }
 
-// Of `tiles` tiles of 128 x 128, how many to work on as such: two are on a
-// CU at a time, 512 on the card.  A last round of up to three quarters of
-// that ends sooner as four times as many tiles of 64 x 64 (fp32, us: 36
-// tiles of 1000 x 2048, 485 as such and 191 as 64s; the 256 of 2048 x 2048,
-// 859 and 721).
+// Of `tiles` tiles of 128 x 128, all with the same sum, how many to work on as
+// such: a round is one on each of 256 CUs.  A last round of up to two thirds
+// ends sooner as four times as many tiles of 64 x 64 (fp32, us, as tiles of
+// 128 and of 64: the 128 of 1000 x 2048 252 and 222, 320 of 2048 x 2560 790
+// and 754, 256 of 2048 x 2048 632 and 651, 253 of X X^T at 2816 x 2816 1272
+// and 1377).
 int64_t big_tiles(int64_t tiles) {
-  const int64_t left = tiles % 512;
-  return left <= 384 ? tiles - left : tiles;
+  const int64_t left = tiles % 256;
+  return left <= 171 ? tiles - left : tiles;
+}
+
+// In a plan the sums differ, and a round of two tiles on each CU ends with its
+// longest: whole rounds only, and of the symmetric products, where they last
+// longest, none in one round (us a step: the 241 of ResNet-50 1015 and 793,
+// 394 of ResNet-101 1306 and 1147, 523 of ResNet-152 1545 and 1415; but 723
+// of three ResNet-50 2100 and 2196).
+int64_t plan_big_tiles(int64_t tiles, bool sym) {
+  return sym && tiles < 640 ? 0 : tiles - tiles % 512;
 }
 
 // Such a matrix needs no workspace.
@@ -1203,7 +1213,9 @@ extern "C" {
 
 int sgp_ns_chunk() { return CHUNK; }
 
-int64_t sgp_ns_big_tiles(int64_t tiles) { return big_tiles(tiles); }
+int64_t sgp_ns_plan_big_tiles(int64_t tiles, bool sym) {
+  return plan_big_tiles(tiles, sym);
+}
 
 bool sgp_ns_is_small(int n, int m) { return is_small(n, m); }
 

@@ -142,6 +142,20 @@ def test_batches(batch, rows, cols):
         assert torch.equal(each[i], ops.newton_schulz(flat[i])), i
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tiles_of_both_sizes(dtype):
+    # 20 of 9 x 11 tiles of 64: X X^T in tiles of 128 and a row of 64s, B X
+    # in a round of 128s and the rest in 64s
+    g = strong(560, 700, batch=(20,)).to(dtype)
+    ref = factor(g)
+    out = ops.newton_schulz(g)
+    single = 6 * 12 * 2.0 ** -12 if dtype == torch.bfloat16 else 0.0
+    for i in range(20):
+        err = float((out[i].double() - ref[i]).norm())
+        assert err <= BOUND + rounding(ref[i], dtype) + single * float(
+            ref[i].norm()), i
+
+
 def test_strides():
     g = strong(70, 90, batch=(4,))
     want = ops.newton_schulz(g)
@@ -368,6 +382,20 @@ def test_step_agrees_with_newton_schulz():
         # the two may group their steps differently; each is within BOUND of
         # the definition in the norm, so they are within twice that
         assert float((p[part] + scale * o).norm()) <= 2 * BOUND * scale
+
+
+def test_step_with_tiles_of_both_sizes():
+    # 66 of 512 x 512: more than a round of tiles of 128 of each product
+    n, side = 66, 512
+    plan = ops.MuonPlan([(i * side * side, side, side) for i in range(n)],
+                        n * side * side)
+    p, buf = (torch.zeros(plan.total, device=dev()) for _ in range(2))
+    g = torch.randn(plan.total, device=dev())
+    ops.muon_step_(p, g, buf, plan, 1.0, nesterov=False)
+    o = ops.newton_schulz(g.view(n, side, side))
+    for i in range(n):
+        # both are within BOUND of the definition
+        assert float((p.view_as(o)[i] + o[i]).norm()) <= 2 * BOUND, i
 
 
 def test_optimizer_against_cpu():
