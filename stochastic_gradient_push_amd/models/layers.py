@@ -423,6 +423,11 @@ class FusedLayerNorm(nn.LayerNorm):
                 f"FusedLayerNorm over {self.normalized_shape} got an input "
                 f"of shape {tuple(x.shape)}"
             )
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError(
+                f"FusedLayerNorm: the residual has shape "
+                f"{tuple(residual.shape)}, the input {tuple(x.shape)}"
+            )
         y = _o.layer_norm(
             x.flatten(-dims),
             None if self.weight is None else self.weight.flatten(),

@@ -94,6 +94,12 @@ def test_module_matches_stock():
         bare(torch.randn(2, 23))
 
 
+def test_module_refuses_another_residual():
+    # as many values in a row, but not the input's
+    with pytest.raises(ValueError, match="residual"):
+        FusedLayerNorm((4, 6))(torch.randn(3, 4, 6), torch.randn(3, 6, 4))
+
+
 @pytest.mark.parametrize("channels_last", [False, True])
 def test_module_2d(channels_last):
     torch.manual_seed(2)
