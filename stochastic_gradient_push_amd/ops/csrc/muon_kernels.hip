@@ -34,9 +34,10 @@
 // and B grows with it.  Values are therefore held as two fp16 numbers,
 // v = hi + lo (22 bits), and a product is hi hi + hi lo + lo hi, three
 // matrix instructions with fp32 accumulation: errors are those of products
-// in fp32 or below (1000 x 2048: 1.0e-6 against 3.2e-6).  Where the result
-// is bf16 the last steps, whose roundings can hardly grow any more, keep hi
-// alone; the host says from which step on.
+// in fp32 or below (1000 x 2048: 1.0e-6 against 3.2e-6).  The last steps of
+// a bf16 result, whose roundings can hardly grow any more, may keep hi alone:
+// only where the caller has asked for it, and the host says from which step
+// on.
 //
 // Scales.  fp16 has a narrow range, so X is stored times 2^e, with e from
 // n m such that its entries are around 1, A times 2^11, B times 2^10; powers

@@ -49,12 +49,12 @@ def _growth(coefficients: Tuple[float, float, float], steps: int) -> float:
 
 
 def _split_steps(steps: int, growth: float, dtype: torch.dtype) -> int:
-    """How many steps need two fp16 numbers for a value.  A rounding to one
-    (2^-11) grows by at most ``growth`` in its own step and in every one that
-    follows.  16 of them together, all at their largest, are twice the
-    rounding of a bf16 result (2^-8); in norm they stay below it (measured
-    0.6 of it for noise, 0.95 for a few strong directions).  fp16 and fp32
-    results need every step."""
+    """How many steps need two fp16 numbers for a value where a caller asks
+    for reduced ones.  A rounding to one (2^-11) grows by at most ``growth``
+    in its own step and in every one that follows.  16 of them together, all
+    at their largest, are twice the rounding of a bf16 result (2^-8); in norm
+    they stay below it (measured 0.6 of it for noise, 0.95 for a few strong
+    directions).  fp16 and fp32 results need every step."""
     if dtype != torch.bfloat16:
         return steps
     single, total = 0, growth
@@ -105,16 +105,19 @@ def newton_schulz(
     steps: int = 5,
     coefficients: Sequence[float] = COEFFICIENTS,
     eps: float = 1e-7,
+    reduced: bool = False,
 ) -> torch.Tensor:
     """``U V^T``, approximately, of a matrix ``[rows, cols]`` or a batch
     ``[..., rows, cols]`` in fp32, bf16 or fp16; contiguous, of ``g``'s
     shape and dtype.
 
     With the usual coefficients five steps bring every singular value above
-    about 1e-3 of the matrix's norm into [0.68, 1.21].  fp32 and fp16
-    results have fp32's accuracy before the last rounding, bf16 results an
-    error of the size of their rounding.  A matrix of zeros stays one; one
-    with a NaN or an infinity becomes NaN as a whole.  Not differentiable.
+    about 1e-3 of the matrix's norm into [0.68, 1.21].  Results have fp32's
+    accuracy and are rounded once.  ``reduced`` lets the last steps of a bf16
+    result keep 11 bits on the device, which adds an error of up to its
+    rounding's size (0.6 of it for noise) and takes a quarter off the time of
+    large matrices; it does nothing elsewhere.  A matrix of zeros stays one;
+    one with a NaN or an infinity becomes NaN as a whole.  Not differentiable.
     """
     if g.dim() < 2:
         raise ValueError("newton_schulz: g must be a matrix or a batch of "
@@ -135,7 +138,7 @@ def newton_schulz(
     rows, cols = g.shape[-2:]
     out = _ext_for(g).newton_schulz(
         g.contiguous().view(g.shape[:-2].numel(), rows, cols), steps,
-        _split_steps(steps, growth, g.dtype),
+        _split_steps(steps, growth, g.dtype) if reduced else steps,
         _group(growth, 2 if g.dtype == torch.float32 else 3), *coefficients,
         growth, eps,
     )

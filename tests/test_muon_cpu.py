@@ -254,3 +254,10 @@ def test_trainer_refuses_muon_without_flat_parameters(tmp_path):
     with pytest.raises(subprocess.CalledProcessError):
         _run_trainer(tmp_path, ["--optimizer", "muon", "--fused_sgd",
                                 "False"])
+
+
+def test_reduced_is_for_the_device():
+    g = torch.randn(6, 10)
+    for dtype in (torch.float32, torch.bfloat16):
+        assert torch.equal(ops.newton_schulz(g.to(dtype), reduced=True),
+                           ops.newton_schulz(g.to(dtype)))

@@ -547,3 +547,52 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in out[i])
+
+
+def plain_error(g):
+    """How far the formulas in fp32 are from the definition, and that."""
+    ref = factor(g)
+    x = g.float()
+    x = x.mT.contiguous() if g.shape[0] > g.shape[1] else x
+    x = x / (x.norm() + 1e-7)
+    a, b, c = COEF
+    for _ in range(5):
+        s = x @ x.T
+        x = a * x + (b * s + c * (s @ s)) @ x
+    x = x.mT if g.shape[0] > g.shape[1] else x
+    return float((x.double() - ref).norm()), ref
+
+
+# one block, tiles of 64, steps in groups, tiles of 128
+@pytest.mark.parametrize("shape", [(60, 90), (300, 700), (90, 400),
+                                   (1100, 257), (2100, 2200)])
+def test_bf16_results_are_rounded_once(shape):
+    """A result that is fp32's and then rounded is the rounded definition but
+    where the border between two values lies in between.  A value off by d is
+    on the wrong side with probability d / step, and then off by a step (at
+    most 2^-7 of it), so the sum of the squares is about sum(d step), at most
+    the product of the norms.  d as for fp32 results: four times that of
+    fp32's formulas; twice all that for chance."""
+    torch.manual_seed(sum(shape))
+    g = torch.randn(*shape, device=dev()).bfloat16()
+    plain, ref = plain_error(g)
+    d = 4 * plain + 4 * 2.0 ** -24 * float(ref.norm())
+    off = float((ops.newton_schulz(g).double()
+                 - ref.bfloat16().double()).norm())
+    assert off ** 2 <= 2 * d * 2.0 ** -7 * float(ref.norm()), (
+        off / float(ref.norm()), plain)
+
+
+@pytest.mark.parametrize("shape", [(60, 90), (300, 700)])
+def test_reduced_steps_are_a_choice(shape):
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        g = strong(*shape, seed=sum(shape)).to(dtype)
+        full, reduced = (ops.newton_schulz(g, reduced=r)
+                         for r in (False, True))
+        # only bf16 results can do with fewer bits
+        assert torch.equal(full, reduced) == (dtype != torch.bfloat16)
+        ref = factor(g)
+        err = float((reduced.double() - ref).norm())
+        assert err <= BOUND + rounding(ref, dtype) + (
+            6 * 12 * 2.0 ** -12 * float(ref.norm())
+            if dtype == torch.bfloat16 else 0.0)
