@@ -20,8 +20,8 @@ int sgp_layer_norm_partials(int dtype, int64_t M, int C);
 void sgp_layer_norm_bwd(int dtype, const void* dy, int64_t ds, const void* x,
                         int64_t xs, const void* y, const void* w, bool w32,
                         const float* mean, const float* rstd, void* dx,
-                        void* dres, float* partials, void* dw, void* db,
-                        bool g32, int64_t M, int C, hipStream_t s);
+                        void* dres, float* partials, int P, void* dw,
+                        void* db, bool g32, int64_t M, int C, hipStream_t s);
 }
 
 namespace {
@@ -152,10 +152,11 @@ layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x,
   }
   if (need_dw) dw = torch::empty({C}, vec);
   if (need_db) db = torch::empty({C}, vec);
+  // the grid, and with it the rows of partial sums: asked for once
+  const int P = sgp_layer_norm_partials(dtype, M, (int)C);
   if (need_dw || need_db)
-    partials = torch::empty(
-        {(int64_t)sgp_layer_norm_partials(dtype, M, (int)C) * 2 * C},
-        x.options().dtype(torch::kFloat32));
+    partials = torch::empty({(int64_t)P * 2 * C},
+                            x.options().dtype(torch::kFloat32));
   sgp_layer_norm_bwd(
       dtype, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), ptr(y),
       ptr(weight),
@@ -163,7 +164,7 @@ layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x,
       mean.data_ptr<float>(), rstd.data_ptr<float>(),
       need_dx ? dx.data_ptr() : nullptr,
       need_dres ? dres.data_ptr() : nullptr,
-      partials.defined() ? partials.data_ptr<float>() : nullptr,
+      partials.defined() ? partials.data_ptr<float>() : nullptr, P,
       need_dw ? dw.data_ptr() : nullptr, need_db ? db.data_ptr() : nullptr,
       g32, M, (int)C,
       c10::hip::getCurrentHIPStream(x.device().index()).stream());

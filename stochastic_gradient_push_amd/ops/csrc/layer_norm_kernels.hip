@@ -609,15 +609,14 @@ int partial_rows(int64_t M, int C) {
 template <typename T>
 void bwd(const void* dy, int64_t ds, const void* x, int64_t xs,
          const void* y, const void* w, bool w32, const float* mean,
-         const float* rstd, void* dx, void* dres, float* partials, void* dw,
-         void* db, bool g32, int64_t M, int C, hipStream_t s) {
+         const float* rstd, void* dx, void* dres, float* partials, int P,
+         void* dw, void* db, bool g32, int64_t M, int C, hipStream_t s) {
   const int nv = vectors<T>(C);
   const T* xp = static_cast<const T*>(x);
   const T* dp = static_cast<const T*>(dy);
   const T* yp = static_cast<const T*>(y);
   T* dxp = static_cast<T*>(dx);
   T* drp = static_cast<T*>(dres);
-  const int P = partial_rows<T>(M, C);
   if (nv > MAX_VECTORS) {
     if (dx != nullptr || dres != nullptr) {
       const int grid = (int)(M < 512 ? M : 512);
@@ -650,7 +649,8 @@ void bwd(const void* dy, int64_t ds, const void* x, int64_t xs,
 
 // dtype: 0 fp32, 1 bf16, 2 fp16.  w32 / g32: weights (their gradients) are
 // fp32 rather than in the rows' type.  Any of res, w, b, mean, y, dx, dres,
-// partials, dw and db may be null.  M and C are positive.
+// partials, dw and db may be null.  M and C are positive.  P, the backward
+// grid, is what sgp_layer_norm_partials has given; partials has P rows of 2 C.
 extern "C" {
 
 void sgp_layer_norm_fwd(int dtype, const void* x, int64_t xs,
@@ -663,17 +663,19 @@ void sgp_layer_norm_fwd(int dtype, const void* x, int64_t xs,
 }
 
 int sgp_layer_norm_partials(int dtype, int64_t M, int C) {
-  return dtype == 0 ? partial_rows<float>(M, C) : partial_rows<__bf16>(M, C);
+  return dtype == 0   ? partial_rows<float>(M, C)
+         : dtype == 1 ? partial_rows<__bf16>(M, C)
+                      : partial_rows<_Float16>(M, C);
 }
 
 void sgp_layer_norm_bwd(int dtype, const void* dy, int64_t ds, const void* x,
                         int64_t xs, const void* y, const void* w, bool w32,
                         const float* mean, const float* rstd, void* dx,
-                        void* dres, float* partials, void* dw, void* db,
-                        bool g32, int64_t M, int C, hipStream_t s) {
+                        void* dres, float* partials, int P, void* dw,
+                        void* db, bool g32, int64_t M, int C, hipStream_t s) {
   auto f = dtype == 0 ? bwd<float> : dtype == 1 ? bwd<__bf16> : bwd<_Float16>;
-  f(dy, ds, x, xs, y, w, w32, mean, rstd, dx, dres, partials, dw, db, g32, M,
-    C, s);
+  f(dy, ds, x, xs, y, w, w32, mean, rstd, dx, dres, partials, P, dw, db, g32,
+    M, C, s);
 }
 
 }  // extern "C"

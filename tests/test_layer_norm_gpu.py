@@ -431,3 +431,16 @@ def test_module_over_two_dimensions():
     assert float((y.double() - ref).abs().max()) <= 256 * U * 4
     y.sum().backward()
     assert norm.weight.grad.shape == (6, 10)
+
+
+@pytest.mark.parametrize("rows,cols", [(100352, 256), (300_000, 24),
+                                       (40_000, 1000)])
+def test_fp16_rows_fill_the_card(rows, cols):
+    # as many blocks as the card holds of this very kernel, each with a row
+    # of partial sums
+    x, w, b, res, dy = inputs(rows, cols, torch.float16, torch.float32, True,
+                              True)
+    got = run(x, w, b, res, True, dy)
+    want = formulas(x, w, b, 1e-5, res, True, dy)
+    for name in want:
+        check(got[name], want[name], name)
