@@ -10,6 +10,8 @@
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
+#include "call_checks.h"
+
 extern "C" {
 void sgp_layer_norm_fwd(int dtype, const void* x, int64_t xs,
                         const void* res, int64_t rs, const void* w,
@@ -54,6 +56,7 @@ void check_rows(const torch::Tensor& t, const char* name,
   TORCH_CHECK(t.numel() == 0 || t.size(1) == 1 || t.stride(1) == 1,
               "layer_norm: ", name,
               " must have contiguous rows");
+  check_memory("layer_norm", t);
 }
 
 void check_vector(const torch::Tensor& t, const char* name,
@@ -66,6 +69,7 @@ void check_vector(const torch::Tensor& t, const char* name,
   TORCH_CHECK(t.scalar_type() == torch::kFloat32
               || t.scalar_type() == x.scalar_type(),
               "layer_norm: ", name, " must be fp32 or have x's dtype");
+  check_memory("layer_norm", t);
 }
 
 const void* ptr(const OptTensor& t) {
@@ -99,6 +103,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_fwd(
   const c10::DeviceGuard guard(x.device());
   const int64_t M = x.size(0);
   torch::Tensor y = torch::empty({M, x.size(1)}, x.options());
+  check_memory("layer_norm", y);  // under a mode that makes such tensors
   torch::Tensor mean, rstd;
   if (statistics) {
     mean = torch::empty({M}, x.options().dtype(torch::kFloat32));
@@ -135,10 +140,12 @@ layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x,
   }
   if (weight.has_value()) check_vector(*weight, "weight", x);
   const int64_t M = x.size(0), C = x.size(1);
-  for (const torch::Tensor& t : {mean, rstd})
+  for (const torch::Tensor& t : {mean, rstd}) {
     TORCH_CHECK(t.is_cuda() && t.device() == x.device() && t.is_contiguous()
                 && t.scalar_type() == torch::kFloat32 && t.numel() == M,
                 "layer_norm: the statistics must be fp32 [M] on x's device");
+    check_memory("layer_norm", t);
+  }
   const c10::DeviceGuard guard(x.device());
   const bool g32 = vectors_fp32 || dtype == 0;
   const auto vec = g32 ? x.options().dtype(torch::kFloat32) : x.options();
@@ -157,6 +164,8 @@ layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x,
   if (need_dw || need_db)
     partials = torch::empty({(int64_t)P * 2 * C},
                             x.options().dtype(torch::kFloat32));
+  for (const torch::Tensor& t : {dx, dres, dw, db, partials})
+    if (t.defined()) check_memory("layer_norm", t);
   sgp_layer_norm_bwd(
       dtype, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), ptr(y),
       ptr(weight),

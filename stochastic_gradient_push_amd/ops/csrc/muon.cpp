@@ -12,6 +12,8 @@
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
+#include "call_checks.h"
+
 extern "C" {
 int sgp_ns_chunk();
 int64_t sgp_ns_plan_big_tiles(int64_t tiles, bool sym);
@@ -102,11 +104,13 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
               "newton_schulz: g must be a contiguous [batch, rows, cols] "
               "device tensor");
   const int dtype = dtype_code(g, "newton_schulz: g");
+  check_memory("newton_schulz", g);
   TORCH_CHECK(steps >= 1 && steps <= 100 && split_steps >= 0
               && split_steps <= steps && group >= 1,
               "newton_schulz: steps out of range");
   const c10::DeviceGuard guard(g.device());
   torch::Tensor out = torch::empty_like(g);
+  check_memory("newton_schulz", out);  // under a mode that makes such tensors
   if (g.numel() == 0) return out;
   const int64_t batch = g.size(0);
   check_matrix(g.size(1), g.size(2));
@@ -281,6 +285,7 @@ void check_flat(const torch::Tensor& t, const char* name,
               && t.scalar_type() == dtype, "muon_step_: ", name,
               " must be a contiguous ", dtype, " vector of ", p.numel(),
               " values on the parameters' device");
+  check_memory("muon_step_", t);
 }
 
 void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
@@ -305,6 +310,8 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
               && lr.scalar_type() == torch::kFloat32,
               "muon_step_: lr must be one fp32 value on the parameters' "
               "device");
+  check_memory("muon_step_", lr);
+  check_memory("muon_step_", tables);
   TORCH_CHECK(tables.device() == p.device(),
               "muon_step_: the plan is for another device");
   TORCH_CHECK(layout.size() == 9, "muon_step_: not a plan");
@@ -317,6 +324,9 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
   torch::Tensor partials = torch::empty({std::max<int64_t>(1, layout[1])},
                                         opt.dtype(torch::kFloat64));
   torch::Tensor r = torch::empty({std::max<int64_t>(1, layout[0])}, opt);
+  // under a mode that makes such tensors
+  for (const torch::Tensor& t : {work, partials, r})
+    check_memory("muon_step_", t);
   sgp_muon_step(g.scalar_type() == torch::kFloat32 ? 0 : 1,
                 p.data_ptr<float>(), g.data_ptr(), buf.data_ptr<float>(),
                 shadow.has_value() ? shadow->data_ptr() : nullptr,
