@@ -13,3 +13,11 @@ inline void check_memory(const char* op, const at::Tensor& t) {
               ": a tensor has no memory of its own (a wrapper, fake or "
               "functional tensor)");
 }
+
+// The kernels compute values only.  A dual tensor's tangent would be gone
+// without a word: it does not show in requires_grad.
+inline void check_tangent(const char* op, const at::Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), op,
+              ": no forward-mode derivative on the device; detach() drops "
+              "the tangent");
+}

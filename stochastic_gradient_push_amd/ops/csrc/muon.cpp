@@ -100,6 +100,7 @@ hipStream_t stream_of(const torch::Tensor& t) {
 torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
                             int64_t split_steps, int64_t group, double a,
                             double b, double c, double growth, double eps) {
+  check_tangent("newton_schulz", g);
   TORCH_CHECK(g.is_cuda() && g.is_contiguous() && g.dim() == 3,
               "newton_schulz: g must be a contiguous [batch, rows, cols] "
               "device tensor");
@@ -295,6 +296,9 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
                 const torch::Tensor& lr, double momentum, double weight_decay,
                 double rest_lr, bool nesterov, int64_t steps, int64_t group,
                 double a, double b, double c, double growth, double eps) {
+  for (const torch::Tensor& t : {p, g, buf, lr})
+    check_tangent("muon_step_", t);
+  if (shadow.has_value()) check_tangent("muon_step_", *shadow);
   check_flat(p, "params", p, torch::kFloat32);
   TORCH_CHECK(p.numel() == total, "muon_step_: the plan is for ", total,
               " values, params has ", p.numel());

@@ -63,3 +63,34 @@ def test_tensors_without_memory(make):
 def test_public_entry_points_refuse_them_too():
     with pytest.raises(RuntimeError, match="no memory"):
         ops.layer_norm(Wrapper(4, 8))
+
+
+@needs_ext
+def test_tangents():
+    """A dual tensor is refused for its tangent before it is refused for
+    where it lies."""
+    import torch.autograd.forward_ad as fwd
+
+    none = "forward-mode"
+    x, v = torch.randn(4, 8), torch.randn(8)
+    tables, layout = ext.muon_plan([(0, 4, 6, 1.0)], 24)
+    with fwd.dual_level():
+        for i in range(4):
+            args = [x, v, v, x.clone()]
+            args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError, match=none):
+                ext.layer_norm(*args[:3], 1e-5, args[3], False)
+        with pytest.raises(RuntimeError, match=none):
+            ext.newton_schulz(fwd.make_dual(torch.ones(1, 4, 6),
+                                            torch.ones(1, 4, 6)),
+                              5, 5, 1, *COEF, 4.0, 1e-7)
+        for i in range(5):
+            args = [torch.ones(24) for _ in range(4)] + [torch.ones(1)]
+            args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            p, g, buf, shadow, lr = args
+            with pytest.raises(RuntimeError, match=none):
+                ext.muon_step_(p, g, buf, shadow, tables, layout, 24, lr,
+                               0.9, 0.0, 1.0, True, 5, 1, *COEF, 4.0, 1e-7)
+        # the host's path differentiates
+        y = ops.layer_norm(fwd.make_dual(x, torch.ones_like(x) * x), v)
+        assert fwd.unpack_dual(y).tangent is not None

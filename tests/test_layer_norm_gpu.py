@@ -444,3 +444,37 @@ def test_fp16_rows_fill_the_card(rows, cols):
     want = formulas(x, w, b, 1e-5, res, True, dy)
     for name in want:
         check(got[name], want[name], name)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    x, res = torch.randn(4, 8, device=dev()), torch.randn(4, 8, device=dev())
+    w, b = torch.randn(8, device=dev()), torch.randn(8, device=dev())
+    args = [x, w, b, res]
+    with fwd.dual_level():
+        for i in range(4):
+            some = list(args)
+            some[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            for grad in (False, True):
+                some[0] = some[0] if i == 0 else x.clone().requires_grad_(grad)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    ops.layer_norm(some[0], some[1], some[2],
+                                   residual=some[3])
+        # a tangent that comes with the output's gradient
+        leaf = x.clone().requires_grad_(True)
+        y = ops.layer_norm(leaf, w, b)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, fwd.make_dual(res, x))
+        # one that was left behind is no hindrance
+        dual = fwd.make_dual(x, res)
+        assert torch.equal(ops.layer_norm(dual.detach(), w, b),
+                           ops.layer_norm(x, w, b))
+    for call in (
+        lambda: torch.func.jvp(lambda t: ops.layer_norm(t, w, b), (x,),
+                               (res,)),
+        lambda: torch.func.vmap(lambda t: ops.layer_norm(t, w, b))(x),
+        lambda: torch.func.grad(lambda t: ops.layer_norm(t, w, b).sum())(x),
+    ):
+        with pytest.raises(RuntimeError):
+            call()

@@ -596,3 +596,24 @@ def test_reduced_steps_are_a_choice(shape):
         assert err <= BOUND + rounding(ref, dtype) + (
             6 * 12 * 2.0 ** -12 * float(ref.norm())
             if dtype == torch.bfloat16 else 0.0)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    g = torch.randn(4, 6, device=dev())
+    plan = ops.MuonPlan([(0, 4, 6)], 24, "cuda")
+    with fwd.dual_level():
+        dual = fwd.make_dual(g, torch.ones_like(g))
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad), \
+                    pytest.raises(RuntimeError, match="forward-mode"):
+                ops.newton_schulz(dual)
+        ops.newton_schulz(dual.detach())
+        flat = [g.flatten().clone() for _ in range(3)]
+        for i in range(3):
+            some = list(flat)
+            some[i] = dual.flatten()
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.muon_step_(*some, plan, 0.1)
+        assert all(torch.equal(t, g.flatten()) for t in flat)
