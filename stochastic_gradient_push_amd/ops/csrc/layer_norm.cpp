@@ -224,6 +224,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
     const torch::Tensor &x = saved[0], &weight = saved[1], &mean = saved[2],
                         &rstd = saved[3], &y = saved[4];
     const torch::Tensor& dy = grads[0];
+    check_untraced("layer_norm");
     check_tangent("layer_norm", dy);
     const int64_t flags = ctx->saved_data["flags"].toInt();
     // numbered over the tensors that there are
@@ -266,6 +267,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 torch::Tensor layer_norm(const torch::Tensor& x, const OptTensor& weight,
                          const OptTensor& bias, double eps,
                          const OptTensor& res, bool relu) {
+  check_untraced("layer_norm");
   check_tangent("layer_norm", x);
   for (const OptTensor* t : {&weight, &bias, &res})
     if (t->has_value()) check_tangent("layer_norm", **t);

@@ -100,6 +100,7 @@ hipStream_t stream_of(const torch::Tensor& t) {
 torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
                             int64_t split_steps, int64_t group, double a,
                             double b, double c, double growth, double eps) {
+  check_untraced("newton_schulz");
   check_tangent("newton_schulz", g);
   TORCH_CHECK(g.is_cuda() && g.is_contiguous() && g.dim() == 3,
               "newton_schulz: g must be a contiguous [batch, rows, cols] "
@@ -296,6 +297,7 @@ void muon_step_(torch::Tensor p, const torch::Tensor& g, torch::Tensor buf,
                 const torch::Tensor& lr, double momentum, double weight_decay,
                 double rest_lr, bool nesterov, int64_t steps, int64_t group,
                 double a, double b, double c, double growth, double eps) {
+  check_untraced("muon_step_");
   for (const torch::Tensor& t : {p, g, buf, lr})
     check_tangent("muon_step_", t);
   if (shadow.has_value()) check_tangent("muon_step_", *shadow);

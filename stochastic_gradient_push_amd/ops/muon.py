@@ -118,7 +118,8 @@ def newton_schulz(
     rounding's size (0.6 of it for noise) and takes a quarter off the time of
     large matrices; it does nothing elsewhere.  A matrix of zeros stays one;
     one with a NaN or an infinity becomes NaN as a whole.  Not differentiable:
-    a ``g`` that requires a gradient is refused, on the device a dual one too.
+    a ``g`` that requires a gradient is refused, on the device a dual one and
+    a call under ``torch.jit.trace`` or ``make_fx`` too.
     """
     if g.dim() < 2:
         raise ValueError("newton_schulz: g must be a matrix or a batch of "
@@ -212,7 +213,7 @@ def muon_step_(
       g = g + weight_decay * p;  buf, u as above;  p = p - lr * u
     ``shadow``, where given, receives the new parameters in bf16.  ``lr`` is
     a float, or one value on the device that a captured step reads anew.
-    Not recorded by autograd; the device refuses dual tensors.
+    Not recorded by autograd; the device refuses dual tensors and tracing.
     """
     coefficients = _check_numbers("muon_step_", steps, coefficients, eps)
     growth = _growth(coefficients, steps)

@@ -31,8 +31,9 @@ def layer_norm(
     left out; ``residual`` has ``x``'s shape and dtype.  Arithmetic is fp32
     throughout, rounded once.  Differentiable once in ``x``, ``weight``,
     ``bias`` and ``residual``, on the device in reverse mode only (a dual
-    tensor is refused); the vectors' gradients are summed in a fixed order.
-    A row with a NaN or an infinity gives a row of NaN.
+    tensor is refused, and so is a call under ``torch.jit.trace`` or
+    ``make_fx``); the vectors' gradients are summed in a fixed order.  A row
+    with a NaN or an infinity gives a row of NaN.
     """
     if x.dtype not in _DTYPES:
         raise TypeError(f"layer_norm: x must be fp32, bf16 or fp16, got "

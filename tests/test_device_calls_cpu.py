@@ -94,3 +94,34 @@ def test_tangents():
         # the host's path differentiates
         y = ops.layer_norm(fwd.make_dual(x, torch.ones_like(x) * x), v)
         assert fwd.unpack_dual(y).tangent is not None
+
+
+@needs_ext
+@pytest.mark.filterwarnings("ignore")
+def test_tracing():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    tables, layout = ext.muon_plan([(0, 4, 6, 1.0)], 24)
+
+    def norm(t):
+        return ext.layer_norm(t, None, None, 1e-5, None, False)
+
+    def orthogonal(t):
+        return ext.newton_schulz(t[None], 5, 5, 1, *COEF, 4.0, 1e-7)
+
+    def step(t):
+        t = t.flatten()
+        ext.muon_step_(t, t, t, None, tables, layout, 24, t[:1], 0.9, 0.0,
+                       1.0, True, 5, 1, *COEF, 4.0, 1e-7)
+        return t
+
+    x = torch.randn(4, 6)
+    for f in (norm, orthogonal, step):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (x,))
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(f)(x)
+    # the host's path can be
+    traced = torch.jit.trace(ops.layer_norm, (x,))
+    y = torch.randn(4, 6)
+    assert torch.allclose(traced(y), ops.layer_norm(y), atol=1e-6)

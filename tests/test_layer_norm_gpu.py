@@ -478,3 +478,18 @@ def test_forward_mode_is_refused():
     ):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_tracing_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(4, 8, device=dev())
+    for grad in (False, True):
+        leaf = x.clone().requires_grad_(grad)
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda t: ops.layer_norm(t), (leaf,))
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(lambda t: ops.layer_norm(t))(x)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(FusedLayerNorm2d(6).to(dev()),
+                        (torch.randn(2, 6, 3, 3, device=dev()),))

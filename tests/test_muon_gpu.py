@@ -617,3 +617,23 @@ def test_forward_mode_is_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 ops.muon_step_(*some, plan, 0.1)
         assert all(torch.equal(t, g.flatten()) for t in flat)
+
+
+def test_tracing_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    g = torch.randn(4, 6, device=dev())
+    plan = ops.MuonPlan([(0, 4, 6)], 24, "cuda")
+    flat = [g.flatten().clone() for _ in range(3)]
+
+    def step(p, grads, buf):
+        ops.muon_step_(p, grads, buf, plan, torch.ones(1, device=dev()))
+        return p
+
+    for trace in (lambda f, a: torch.jit.trace(f, a),
+                  lambda f, a: make_fx(f)(*a)):
+        with pytest.raises(RuntimeError, match="traced"):
+            trace(lambda t: ops.newton_schulz(t), (g,))
+        with pytest.raises(RuntimeError, match="traced"):
+            trace(step, tuple(flat))
+    assert all(torch.equal(t, g.flatten()) for t in flat)
