@@ -89,10 +89,13 @@ void check_size(const torch::Tensor& x) {
               "layer_norm: the last dimension must be 1 to 2^30 long");
 }
 
-// -> (y [M, C], mean [M], rstd [M]); the statistics only if asked for
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_fwd(
+// x: [M, C] -> (y, mean [M], rstd [M]); the statistics only if asked for.  y
+// is made with the sizes that the caller shows: a view of it, made where
+// autograd does not look, could not be changed in place.
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> forward_rows(
     const torch::Tensor& x, const OptTensor& weight, const OptTensor& bias,
-    const OptTensor& res, double eps, bool relu, bool statistics) {
+    const OptTensor& res, double eps, bool relu, bool statistics,
+    at::IntArrayRef sizes) {
   check_rows(x, "x", x);
   const int dtype = dtype_code(x);
   check_size(x);
@@ -102,7 +105,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_fwd(
   const bool w32 = is_fp32(weight, bias);
   const c10::DeviceGuard guard(x.device());
   const int64_t M = x.size(0);
-  torch::Tensor y = torch::empty({M, x.size(1)}, x.options());
+  torch::Tensor y = torch::empty(sizes, x.options());
   check_memory("layer_norm", y);  // under a mode that makes such tensors
   torch::Tensor mean, rstd;
   if (statistics) {
@@ -120,6 +123,12 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_fwd(
     C10_HIP_CHECK(hipGetLastError());
   }
   return {y, mean, rstd};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_fwd(
+    const torch::Tensor& x, const OptTensor& weight, const OptTensor& bias,
+    const OptTensor& res, double eps, bool relu, bool statistics) {
+  return forward_rows(x, weight, bias, res, eps, relu, statistics, x.sizes());
 }
 
 // -> (dx, dres, dw, db), each only if asked for.  `y`: the output, if there
@@ -202,9 +211,8 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
                                const torch::Tensor& x,
                                const OptTensor& weight, const OptTensor& bias,
                                const OptTensor& res, double eps, bool relu) {
-    auto [y, mean, rstd] = layer_norm_fwd(rows(x), weight, bias, rows(res),
-                                          eps, relu, true);
-    y = y.view(x.sizes());
+    auto [y, mean, rstd] = forward_rows(rows(x), weight, bias, rows(res),
+                                        eps, relu, true, x.sizes());
     ctx->save_for_backward({x, weight.value_or(torch::Tensor()), mean, rstd,
                             relu ? y : torch::Tensor()});
     const OptTensor& vector = weight.has_value() ? weight : bias;
@@ -277,8 +285,8 @@ torch::Tensor layer_norm(const torch::Tensor& x, const OptTensor& weight,
   if (torch::GradMode::is_enabled()
       && (x.requires_grad() || wants(weight) || wants(bias) || wants(res)))
     return LayerNorm::apply(x, weight, bias, res, eps, relu);
-  return std::get<0>(layer_norm_fwd(rows(x), weight, bias, rows(res), eps,
-                                    relu, false)).view(x.sizes());
+  return std::get<0>(forward_rows(rows(x), weight, bias, rows(res), eps,
+                                  relu, false, x.sizes()));
 }
 
 }  // namespace

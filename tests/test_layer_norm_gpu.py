@@ -493,3 +493,44 @@ def test_tracing_is_refused():
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(FusedLayerNorm2d(6).to(dev()),
                         (torch.randn(2, 6, 3, 3, device=dev()),))
+
+
+@pytest.mark.parametrize("shape", [(6, 40), (3, 5, 40)])
+def test_output_changed_in_place(shape):
+    torch.manual_seed(0)
+    x = torch.randn(*shape, device=dev())
+    w = torch.randn(40, device=dev())
+    dy = torch.randn_like(x)
+
+    def grads(change):
+        xs, ws = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = change(ops.layer_norm(xs, ws, residual=x))
+        return [y.detach(), *torch.autograd.grad(y, (xs, ws), dy)]
+
+    for inplace, other in (
+        (lambda y: y.mul_(2.0), lambda y: y * 2.0),
+        (lambda y: torch.relu_(y), torch.relu),
+        (lambda y: y.add_(x), lambda y: y + x),
+    ):
+        assert all(torch.equal(a, b)
+                   for a, b in zip(grads(inplace), grads(other)))
+    # the ReLU's output is needed for its gradient
+    xs = x.clone().requires_grad_(True)
+    y = ops.layer_norm(xs, relu=True).mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+def test_modules_outputs_changed_in_place():
+    torch.manual_seed(1)
+    relu = torch.nn.ReLU(inplace=True)
+    for norm, x in ((FusedLayerNorm(24), torch.randn(5, 24)),
+                    (FusedLayerNorm((4, 6)), torch.randn(5, 4, 6)),
+                    (FusedLayerNorm2d(24), torch.randn(2, 24, 3, 5))):
+        norm, x = norm.to(dev()), x.to(dev()).requires_grad_(True)
+        y = relu(norm(x))
+        want = torch.relu(norm(x))
+        assert torch.equal(y, want)
+        got, = torch.autograd.grad(y.sum(), x)
+        ref, = torch.autograd.grad(want.sum(), x)
+        assert torch.equal(got, ref)
