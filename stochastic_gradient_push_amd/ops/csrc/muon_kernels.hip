@@ -426,6 +426,14 @@ __device__ __forceinline__ int x_exp(const Mat& q, float r, int step,
   return shift > 0 ? q.e - shift : q.e;
 }
 
+// What X X^T, of an X that is stored times 2^e, is multiplied with to be A:
+// r^2 2^-2e A_SCALE.  r alone may be 1e-38 and its square 0, but r 2^-e is of
+// the size that r X has at its largest.
+__device__ __forceinline__ float gram_factor(float r, int e) {
+  const float h = ldexpf(r, -e);
+  return h * h * A_SCALE;
+}
+
 __device__ __forceinline__ void load_lds(const half_t* from, half_t* to) {
   __builtin_amdgcn_global_load_lds(
       (const __attribute__((address_space(1))) void*)from,
@@ -723,9 +731,9 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(
   if (MODE == GRAM || MODE == APPLY) {
     const int e = x_exp(q, rr, step, k);
     if (MODE == GRAM)
-      f = ldexpf(rr * rr, -2 * e) * A_SCALE;
+      f = gram_factor(rr, e);
     else if (LAST)
-      f = ldexpf(rr / B_SCALE, -e);
+      f = ldexpf(rr, -e) / B_SCALE;
     else
       f = ldexpf(1.f / B_SCALE, x_exp(q, rr, step + group, k) - e);
   }
@@ -980,13 +988,13 @@ __global__ __launch_bounds__(256) void k_ns_small(
   const int r0 = wave * 16 + (lane >> 4) * 4;
   for (int step = 0; step < steps; ++step) {
     const int e = x_exp(q, r, step, k);
-    const float gram = ldexpf(r * r, -2 * e) * A_SCALE;
+    const float gram = gram_factor(r, e);
     if (step < split_steps)
       small_step<true, MP>(x, xt, a, b, gram, k, acc);
     else
       small_step<false, MP>(x, xt, a, b, gram, k, acc);
     const bool last = step + 1 == steps;
-    const float f = last ? ldexpf(r / B_SCALE, -e)
+    const float f = last ? ldexpf(r, -e) / B_SCALE
                          : ldexpf(1.f / B_SCALE, x_exp(q, r, step + 1, k) - e);
 #pragma unroll
     for (int j = 0; j < MP / 16; ++j) {

@@ -637,3 +637,22 @@ def test_tracing_is_refused():
         with pytest.raises(RuntimeError, match="traced"):
             trace(step, tuple(flat))
     assert all(torch.equal(t, g.flatten()) for t in flat)
+
+
+@pytest.mark.parametrize("shape", [(8, 24), (300, 100), (128, 640),
+                                   (700, 800)])
+def test_far_below_eps_with_many_steps(shape):
+    # r = |G| / (|G| + eps) = 1e-23, whose square fp32 does not hold: values
+    # that have grown to 1 after 85 steps still have to stop there
+    steps, coef = 100, (1.875, -1.25, 0.375)
+    torch.manual_seed(sum(shape))
+    g = torch.randn(*shape, device=dev())
+    g = g * (1e-30 / float(g.norm()))
+    ref = factor(g, steps, coef)
+    out = ops.newton_schulz(g, steps=steps, coefficients=coef)
+    assert bool(torch.isfinite(out).all())
+    # a step's eight roundings are relative to the norm, and grow as the
+    # smallest singular value does
+    s = torch.linalg.svdvals(g.double())
+    bound = steps * 8 * 2.0 ** -23 * float(s.norm() / s.min())
+    assert float((out.double() - ref).norm()) <= bound
