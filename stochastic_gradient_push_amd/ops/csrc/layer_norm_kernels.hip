@@ -215,7 +215,12 @@ __global__ __launch_bounds__(block_of(TPR)) void k_ln_fwd(
   }
 }
 
-// Rows too long for registers: one block each, read three times.
+// Rows too long for registers: one block each, read three times.  A thread
+// may have 2^20 values of a row: it adds up the 4 or 8 of a vector, and the
+// vectors' sums in 64 bits: one after another in 32 bits the mean of 2^26
+// values of 0.1 was off by 6e-4 of itself, and of a row without a variance
+// nothing else is left.  It costs nothing (4096 x 16384 fp32 147 us, both ways
+// 347; 1024 x 65536 bf16 76 and 196).
 template <typename T>
 __global__ __launch_bounds__(1024) void k_ln_fwd_long(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ res,
@@ -227,20 +232,28 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(
   const float inv = 1.f / (float)C;
   for (int64_t r = blockIdx.x; r < M; r += gridDim.x) {
     const T* xr = x + r * xs;
-    float f[N], s = 0.f, q = 0.f;
+    float f[N];
+    double all = 0.0;
     for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
       load<T>(xr, (int)c, C, f);
+      float v = 0.f;
 #pragma unroll
-      for (int j = 0; j < N; ++j) s += f[j];
+      for (int j = 0; j < N; ++j) v += f[j];
+      all += v;
     }
+    float s = (float)all;
     row_sum<1024, 1>(&s, lds);
     const float mean = s / (float)C;  // exact where the sum is
+    all = 0.0;
     for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
       load<T>(xr, (int)c, C, f);
+      float v = 0.f;
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (c + j < C) q += (f[j] - mean) * (f[j] - mean);
+        if (c + j < C) v += (f[j] - mean) * (f[j] - mean);
+      all += v;
     }
+    float q = (float)all;
     row_sum<1024, 1>(&q, lds);
     const float rstd = 1.f / sqrtf(q * inv + eps);
     for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
@@ -403,9 +416,9 @@ __global__ __launch_bounds__(1024) void k_ln_bwd_long(
     const float mu = mean[r], rs = rstd[r];
     float m0 = 0.f, m1 = 0.f;
     for (int pass = 0; pass < 2; ++pass) {
-      float s[2] = {0.f, 0.f};
+      double all[2] = {0.0, 0.0};  // as in k_ln_fwd_long
       for (int64_t c = threadIdx.x * N; c < C; c += 1024 * N) {
-        float h[N], gv[N], wv[N];
+        float h[N], gv[N], wv[N], v[2] = {0.f, 0.f};
         load<T>(x + r * xs, (int)c, C, h);
         load<T>(dy + r * ds, (int)c, C, gv);
         load_w<T>(w, w32, (int)c, C, 1.f, wv);
@@ -421,14 +434,17 @@ __global__ __launch_bounds__(1024) void k_ln_bwd_long(
         for (int j = 0; j < N; ++j) {
           h[j] = (h[j] - mu) * rs;
           gv[j] *= wv[j];
-          s[0] += gv[j];
-          s[1] += gv[j] * h[j];
+          v[0] += gv[j];
+          v[1] += gv[j] * h[j];
           gv[j] = rs * (gv[j] - m0 - h[j] * m1);
         }
+        all[0] += v[0];
+        all[1] += v[1];
         if (pass == 1) store<T>(dx + r * C, (int)c, C, gv);
       }
       if (dx == nullptr) break;
       if (pass == 0) {
+        float s[2] = {(float)all[0], (float)all[1]};
         row_sum<1024, 2>(s, lds);
         m0 = s[0] * inv;
         m1 = s[1] * inv;

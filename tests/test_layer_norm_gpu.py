@@ -534,3 +534,28 @@ def test_modules_outputs_changed_in_place():
         got, = torch.autograd.grad(y.sum(), x)
         ref, = torch.autograd.grad(want.sum(), x)
         assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [24, 600, 3000, 16500])
+def test_constant_long_rows_and_short_ones(cols, dtype):
+    # a mean that is off shows undiminished where the variance is 0
+    x = torch.full((2, cols), 0.1, device=dev()).to(dtype)
+    y = ops.layer_norm(x)
+    assert float(y.abs().max()) <= 48 * U * 0.1 / 1e-5 ** 0.5
+
+
+def test_a_constant_row_of_millions():
+    # 2^16 values a thread: added one after another in 32 bits the mean was
+    # off by up to 2^16 * 2^-25 of itself
+    cols = (1 << 26) + 5
+    x = torch.full((1, cols), 0.1, device=dev())
+    bound = 48 * U * 0.1 / 1e-5 ** 0.5
+    y = ops.layer_norm(x)
+    assert float(y.abs().max()) <= bound
+    # the gradient's sums likewise: of equal values nothing is left
+    leaf = x.requires_grad_(True)
+    w = torch.full((cols,), 0.1, device=dev())
+    dx, = torch.autograd.grad(ops.layer_norm(leaf, w), leaf,
+                              torch.ones_like(x))
+    assert float(dx.abs().max()) <= bound
