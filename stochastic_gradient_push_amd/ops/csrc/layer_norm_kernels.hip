@@ -491,16 +491,16 @@ __global__ __launch_bounds__(256) void k_ln_bwd_cols(
     }
 }
 
-// Column sums of partials [P][2C]: a block has 16 columns and `blockDim.x`
-// / 16 threads on each, which add up in a fixed order.
+// Column sums of partials [P][2C] from column c0 on: a block has 16 columns
+// and `blockDim.x` / 16 threads on each, which add up in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_ln_bwd_sum(
-    const float* __restrict__ partials, int P, int C, void* __restrict__ dw,
-    void* __restrict__ db, bool w32) {
+    const float* __restrict__ partials, int P, int C, int64_t c0,
+    void* __restrict__ dw, void* __restrict__ db, bool w32) {
   __shared__ float lds[1024];
   const int cl = threadIdx.x & 15, k0 = threadIdx.x >> 4;
   const int K = blockDim.x >> 4;
-  const int64_t c = (int64_t)blockIdx.x * 16 + cl, S = 2 * (int64_t)C;
+  const int64_t c = c0 + (int64_t)blockIdx.x * 16 + cl, S = 2 * (int64_t)C;
   float v = 0.f;
   if (c < S) {
     const float* p = partials + c;
@@ -654,11 +654,16 @@ void bwd(const void* dy, int64_t ds, const void* x, int64_t xs,
     LN_FOR_SHAPE(nv, LN_BWD);
 #undef LN_BWD
   }
-  if (partials != nullptr)
-    hipLaunchKernelGGL(k_ln_bwd_sum<T>,
-                       dim3((unsigned)cdiv(2 * (int64_t)C, 16)),
-                       dim3(P > 64 ? 1024 : 256), 0, s, partials, P, C, dw,
-                       db, g32);
+  if (partials == nullptr) return;
+  // 64 or 16 threads a column: a launch of up to 2^31 of the 2^32 threads
+  // that it may have
+  const int64_t S = 2 * (int64_t)C, most = (int64_t(1) << 31) / 64;
+  for (int64_t c0 = 0; c0 < S; c0 += most) {
+    const int64_t cols = S - c0 < most ? S - c0 : most;
+    hipLaunchKernelGGL(k_ln_bwd_sum<T>, dim3((unsigned)cdiv(cols, 16)),
+                       dim3(P > 64 ? 1024 : 256), 0, s, partials, P, C, c0,
+                       dw, db, g32);
+  }
 }
 
 }  // namespace

@@ -559,3 +559,22 @@ def test_a_constant_row_of_millions():
     dx, = torch.autograd.grad(ops.layer_norm(leaf, w), leaf,
                               torch.ones_like(x))
     assert float(dx.abs().max()) <= bound
+
+
+def test_more_columns_than_a_launch_has_threads():
+    # 16 threads a column of dw and of db in the sum over the blocks: 2^32
+    cols = (1 << 27) + 3
+    g = torch.Generator(device=dev()).manual_seed(0)
+    x = torch.randn(1, cols, generator=g, device=dev())
+    dy = torch.randn(1, cols, generator=g, device=dev())
+    w, b = (torch.ones(cols, device=dev(), requires_grad=True)
+            for _ in range(2))
+    dw, db = torch.autograd.grad(ops.layer_norm(x, w, b), (w, b), dy)
+    assert torch.equal(db, dy[0])
+    mean = float(x.mean(dtype=torch.float64))
+    var = float(((x.double() - mean) ** 2).mean())
+    hat = (x[0].double() - mean) / (var + 1e-5) ** 0.5
+    want = dy[0].double() * hat
+    # the mean and the deviation: 24 roundings of values of size 1, as above
+    bound = 8 * U * want.abs() + 64 * U * dy[0].double().abs()
+    assert bool(((dw.double() - want).abs() <= bound).all())
