@@ -119,11 +119,16 @@ torch::Tensor newton_schulz(const torch::Tensor& g, int64_t steps,
   const Mat q = make_mat(0, g.size(1), g.size(2), 1.0);
   const int64_t x_total = batch * q.np * (int64_t)q.mp;
   const int64_t a_total = batch * q.np * (int64_t)q.np;
-  TORCH_CHECK(x_total / 4096 < (int64_t(1) << 31)
-              && batch * q.chunk1 < (int64_t(1) << 31),
+  const bool small = sgp_ns_is_small(q.n, q.m);
+  // matrices and chunks are counted in 32 bits, and a launch has less than
+  // 2^32 threads, 256 a tile or chunk (such a workspace would fill the card
+  // several times); small matrices are launched in parts
+  TORCH_CHECK(batch * q.chunk1 < (int64_t(1) << 31)
+              && (small || (x_total / 4096 < (int64_t(1) << 24)
+                            && batch * q.chunk1 < (int64_t(1) << 24))),
               "newton_schulz: too many values in one call");
   torch::Tensor work, partials, r;
-  if (!sgp_ns_is_small(q.n, q.m)) {
+  if (!small) {
     const auto opt = g.options();
     work = torch::empty({work_size(x_total, a_total)},
                         opt.dtype(torch::kFloat16));
@@ -255,8 +260,9 @@ std::tuple<torch::Tensor, std::vector<int64_t>> muon_plan(
     at = to;
   }
   rest(total);
-  TORCH_CHECK(packs.size() < (size_t(1) << 31)
-              && chunks.size() < (size_t(1) << 31),
+  // a launch has less than 2^32 threads, 256 a tile or chunk
+  TORCH_CHECK(packs.size() < (size_t(1) << 24)
+              && chunks.size() < (size_t(1) << 24),
               "muon: too many values in one plan");
 
   const std::vector<int64_t> layout = {

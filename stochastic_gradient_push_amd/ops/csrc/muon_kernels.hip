@@ -1153,11 +1153,17 @@ void newton_schulz(const T* g, T* out, const Mat& first, int batch, int steps,
                    int split_steps, int group, Coef k, float eps, void* work,
                    double* partials, float* r, hipStream_t s) {
   if (is_small(first.n, first.m)) {
-    const Uniform src{first, batch, 0, 0};
     auto f = first.mp == 64 ? k_ns_small<T, 64>
              : first.mp == 128 ? k_ns_small<T, 128> : k_ns_small<T, 192>;
-    hipLaunchKernelGGL(f, dim3((unsigned)batch), dim3(256), 0, s, src, g, out,
-                       steps, split_steps, k, eps);
+    // a launch has less than 2^32 threads
+    const int most = 1 << 23;
+    for (int64_t at = 0; at < batch; at += most) {
+      const int now = (int)(batch - at < most ? batch - at : most);
+      Uniform src{first, now, 0, 0};
+      src.first.start = at * first.rows * first.cols;
+      hipLaunchKernelGGL(f, dim3((unsigned)now), dim3(256), 0, s, src, g, out,
+                         steps, split_steps, k, eps);
+    }
     return;
   }
   const int64_t nt = first.np / 64, mt = first.mp / 64;

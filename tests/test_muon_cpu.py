@@ -261,3 +261,14 @@ def test_reduced_is_for_the_device():
     for dtype in (torch.float32, torch.bfloat16):
         assert torch.equal(ops.newton_schulz(g.to(dtype), reduced=True),
                            ops.newton_schulz(g.to(dtype)))
+
+
+def test_plan_refuses_more_than_a_launch_holds():
+    # 2^24 chunks of 2048 values, a block of 256 threads each
+    ext = ops._load_extension()
+    if ext is None:
+        pytest.skip("extension not built")
+    with pytest.raises(RuntimeError, match="too many"):
+        ext.muon_plan([], 2048 << 24)
+    tables, layout = ext.muon_plan([(0, 4, 6, 1.0)], 1 << 20)
+    assert layout[1] == 1 + 512 and tables.numel() > 0

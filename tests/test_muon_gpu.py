@@ -656,3 +656,16 @@ def test_far_below_eps_with_many_steps(shape):
     s = torch.linalg.svdvals(g.double())
     bound = steps * 8 * 2.0 ** -23 * float(s.norm() / s.min())
     assert float((out.double() - ref).norm()) <= bound
+
+
+def test_more_matrices_than_a_launch_has_threads():
+    # a block of 256 threads a matrix: 2^32 from 2^24 on
+    batch = (1 << 24) + 5
+    g = torch.zeros(batch, 2, 3, device=dev(), dtype=torch.bfloat16)
+    some = [0, 1, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, batch - 1]
+    for i in some:
+        g[i] = strong(2, 3, seed=i % 97).bfloat16()
+    out = ops.newton_schulz(g)
+    for i in some:
+        assert torch.equal(out[i], ops.newton_schulz(g[i])), i
+    assert int((out != 0).any(-1).any(-1).sum()) == len(some)
