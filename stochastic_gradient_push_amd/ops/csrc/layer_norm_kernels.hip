@@ -5,7 +5,7 @@
 //   hat  = (x - mean) * rstd     rstd = 1 / sqrt(var + eps)
 //   y    = relu(hat * w + b + res)
 //
-//   g    = dy where y > 0        dres = g
+//   g    = dy where the sum is positive, rounded to zero or not;  dres = g
 //   dw   = sum_rows(g * hat)     db   = sum_rows(g)
 //   dx   = rstd * (g w - mean_cols(g w) - hat * mean_cols(g w hat))
 //
@@ -110,6 +110,17 @@ __device__ __forceinline__ void put_w(void* w, bool w32, int64_t c, float f) {
     static_cast<T*>(w)[c] = (T)f;
 }
 
+// max(z, 0); a NaN stays.  The backward pass reads y to know where z was
+// positive, so a positive z that T rounds to zero becomes -0, and +0 means
+// that there is no gradient.
+template <typename T>
+__device__ __forceinline__ float rectify(float z) {
+  return z <= 0.f ? 0.f : (float)(T)z == 0.f ? -0.f : z;
+}
+__device__ __forceinline__ bool was_cut(float y) {
+  return __float_as_uint(y) == 0;
+}
+
 // Sum of K values over the TPR threads of a row, the same in each of them.
 // Up to a wave: butterflies.  Above: a block has one row, its waves meet in
 // `lds` (K * TPR / 64 floats, not touched again before the next barrier).
@@ -204,7 +215,7 @@ __global__ __launch_bounds__(block_of(TPR)) void k_ln_fwd(
       for (int j = 0; j < N; ++j) {
         float z = ((float)now[i][j] - mean) * rstd * wv[i][j] + bv[i][j];
         if (res != nullptr) z += (float)now_res[i][j];
-        f[j] = relu && z <= 0.f ? 0.f : z;  // a NaN stays
+        f[j] = relu ? rectify<T>(z) : z;
       }
       store<T>(y + r * C, (t + i * TPR) * N, C, f);
     }
@@ -266,7 +277,7 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(
       for (int j = 0; j < N; ++j) {
         float z = (f[j] - mean) * rstd * wv[j] + bv[j];
         if (res != nullptr) z += a[j];
-        f[j] = relu && z <= 0.f ? 0.f : z;
+        f[j] = relu ? rectify<T>(z) : z;
       }
       store<T>(y + r * C, (int)c, C, f);
     }
@@ -330,7 +341,7 @@ __global__ __launch_bounds__(block_of(TPR)) void k_ln_bwd(
       if constexpr (RELU)
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          if ((float)next_y[i][j] <= 0.f) gv[i][j] = (T)0.f;
+          if (was_cut((float)next_y[i][j])) gv[i][j] = (T)0.f;
       if (dres != nullptr) {
         const int c = (t + i * TPR) * N;
         if (c + N <= C) {
@@ -426,7 +437,7 @@ __global__ __launch_bounds__(1024) void k_ln_bwd_long(
           float a[N];
           load<T>(y + r * C, (int)c, C, a);
 #pragma unroll
-          for (int j = 0; j < N; ++j) gv[j] = a[j] <= 0.f ? 0.f : gv[j];
+          for (int j = 0; j < N; ++j) gv[j] = was_cut(a[j]) ? 0.f : gv[j];
         }
         if (pass == 0 && dres != nullptr)
           store<T>(dres + r * C, (int)c, C, gv);
@@ -474,7 +485,7 @@ __global__ __launch_bounds__(256) void k_ln_bwd_cols(
       float a[N];
       load<T>(y + r * C, c, C, a);
 #pragma unroll
-      for (int j = 0; j < N; ++j) gv[j] = a[j] <= 0.f ? 0.f : gv[j];
+      for (int j = 0; j < N; ++j) gv[j] = was_cut(a[j]) ? 0.f : gv[j];
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) {

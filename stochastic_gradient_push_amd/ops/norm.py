@@ -33,7 +33,8 @@ def layer_norm(
     ``bias`` and ``residual``, on the device in reverse mode only (a dual
     tensor is refused, and so is a call under ``torch.jit.trace`` or
     ``make_fx``); the vectors' gradients are summed in a fixed order.  A row
-    with a NaN or an infinity gives a row of NaN.
+    with a NaN or an infinity gives a row of NaN.  With ``relu`` a positive
+    sum that the type rounds to zero is -0 on the device: its gradient passes.
     """
     if x.dtype not in _DTYPES:
         raise TypeError(f"layer_norm: x must be fp32, bf16 or fp16, got "

@@ -578,3 +578,24 @@ def test_more_columns_than_a_launch_has_threads():
     # the mean and the deviation: 24 roundings of values of size 1, as above
     bound = 8 * U * want.abs() + 64 * U * dy[0].double().abs()
     assert bool(((dw.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype,tiny", [(torch.float16, 2.0 ** -26),
+                                        (torch.float16, 2.0 ** -25),
+                                        (torch.bfloat16, 2.0 ** -135)])
+@pytest.mark.parametrize("cols", [24, 600, 3000, 16500])
+def test_relu_of_sums_that_round_to_zero(dtype, tiny, cols):
+    # hat is 0, so a column's sum is its bias: positive and too small for
+    # the type, negative likewise, zero
+    x = torch.ones(3, cols, device=dev()).to(dtype)
+    b = torch.tensor([tiny, -tiny, 0.0], device=dev()).repeat(cols // 3 + 1)
+    b = b[:cols].contiguous()
+    res = torch.zeros_like(x).requires_grad_(True)
+    b.requires_grad_(True)
+    y = ops.layer_norm(x, None, b, residual=res, relu=True)
+    assert bool((y == 0).all())
+    dy = torch.ones_like(y)
+    dres, db = torch.autograd.grad(y, (res, b), dy)
+    want = (b.detach() > 0).to(dtype)
+    assert torch.equal(dres, want.expand(3, cols))
+    assert torch.equal(db, 3.0 * want.float())
