@@ -66,6 +66,7 @@ def test_public_entry_points_refuse_them_too():
 
 
 @needs_ext
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_tangents():
     """A dual tensor is refused for its tangent before it is refused for
     where it lies."""

@@ -446,6 +446,7 @@ def test_fp16_rows_fill_the_card(rows, cols):
         check(got[name], want[name], name)
 
 
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_forward_mode_is_refused():
     import torch.autograd.forward_ad as fwd
 
@@ -480,6 +481,7 @@ def test_forward_mode_is_refused():
             call()
 
 
+@pytest.mark.filterwarnings("ignore")
 def test_tracing_is_refused():
     from torch.fx.experimental.proxy_tensor import make_fx
 

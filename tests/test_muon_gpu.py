@@ -598,6 +598,7 @@ def test_reduced_steps_are_a_choice(shape):
             if dtype == torch.bfloat16 else 0.0)
 
 
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_forward_mode_is_refused():
     import torch.autograd.forward_ad as fwd
 
@@ -619,6 +620,7 @@ def test_forward_mode_is_refused():
         assert all(torch.equal(t, g.flatten()) for t in flat)
 
 
+@pytest.mark.filterwarnings("ignore")
 def test_tracing_is_refused():
     from torch.fx.experimental.proxy_tensor import make_fx
 
@@ -669,3 +671,141 @@ def test_more_matrices_than_a_launch_has_threads():
     for i in some:
         assert torch.equal(out[i], ops.newton_schulz(g[i])), i
     assert int((out != 0).any(-1).any(-1).sum()) == len(some)
+
+
+def input_roundings(g):
+    """What roundings of the input do to the result: noise of size d |g|
+    comes out as d |g| f(s) / s for each singular value s, where f(s) <=
+    1.21; four roundings."""
+    s = torch.linalg.svdvals(g.double())
+    return 4 * 1.21 * 2.0 ** -24 * float(
+        s.norm() * s.reciprocal().square().mean().sqrt())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_step_on_noise(dtype):
+    """Steps on noise, as sharp as test_noise_against_fp32: four times the
+    error of the same formulas in fp32, and the roundings of p."""
+    matrices = [(3, 64, 147), (10_000, 256, 64), (30_001, 300, 270),
+                (120_000, 128, 576), (200_003, 512, 640)]
+    total = 600_001
+    torch.manual_seed(4)
+    plan = ops.MuonPlan(matrices, total, "cuda")
+    p, buf = (torch.randn(total, device=dev()) for _ in range(2))
+    g = torch.randn(total, device=dev()).to(dtype)
+    lr, mu, wd = 0.5, 0.9, 0.1
+    for nesterov in (False, True):
+        before, was = p.double(), buf.clone()
+        ops.muon_step_(p, g, buf, plan, lr, momentum=mu, weight_decay=wd,
+                       nesterov=nesterov)
+        # u as the kernel has it: a rounding or two of u are noise too
+        u = mu * was + g.float()
+        u = g.float() + mu * u if nesterov else u
+        for start, rows, cols in matrices:
+            part = slice(start, start + rows * cols)
+            scale = lr * max(1.0, rows / cols) ** 0.5
+            ref_u = u[part].view(rows, cols)
+            plain, ref = plain_error(ref_u)
+            want = before[part] * (1 - lr * wd) - scale * ref.reshape(-1)
+            bound = scale * (4 * plain + input_roundings(ref_u)) \
+                + 8 * 2.0 ** -24 * float(want.norm())
+            assert float((p[part].double() - want).norm()) <= bound, (
+                rows, cols)
+
+
+def check_moves(opt, before):
+    """Every matrix of the plan has made the step that the definition makes
+    of the momentum and gradients that lie in the buffers."""
+    group = opt.param_groups[0]
+    _, plan, grads, _ = opt._plans[0]
+    u = grads.double() + group["momentum"] * opt.momentum_buf[
+        :plan.total].double()
+    keep = 1 - group["lr"] * group["weight_decay"]
+    assert plan.matrices
+    for (start, rows, cols), scale in zip(plan.matrices, plan.scales):
+        part = slice(start, start + rows * cols)
+        was, now = before[part].double(), opt.flatp.flat[part].double()
+        step = (was * keep - now) / (group["lr"] * scale)
+        want = factor(u[part].view(rows, cols)).reshape(-1)
+        # four roundings of parameters, seen through lr
+        bound = BOUND + 4 * 2.0 ** -24 * float(was.norm() + now.norm()) / (
+            group["lr"] * scale)
+        assert float((step - want).norm()) <= bound, (rows, cols)
+        # and that is a step of all directions the gradient has
+        assert float(want.norm()) >= 0.5
+
+
+@pytest.mark.parametrize("capture", [False, True])
+def test_training_moves_every_matrix(capture):
+    torch.manual_seed(8)
+    net = resnet18(num_classes=10, norm="layer").to(dev()).to(
+        memory_format=torch.channels_last)
+    gdp = GossipDataParallel(net, rank=0, world_size=1,
+                             working_dtype=torch.bfloat16)
+    opt = FusedMuon(gdp.flatp, lr=0.02, rest_lr=0.1, weight_decay=0.01,
+                    steal_grads=True)
+    x = torch.randn(4, 3, 64, 64, device=dev()).to(
+        memory_format=torch.channels_last)
+    y = torch.randint(0, 10, (4,), device=dev())
+
+    def step():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = torch.nn.functional.cross_entropy(net(x), y)
+        loss.backward()
+        opt.step()
+        opt.zero_grad()
+        return loss.detach()
+
+    # the last norm of a residual branch starts at 0: no gradient before it
+    for _ in range(2):
+        step()
+    once = step
+    if capture:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        once = graph.replay
+    for _ in range(3):
+        torch.cuda.synchronize()
+        before = opt.flatp.flat.clone()
+        x.normal_()
+        once()
+        torch.cuda.synchronize()
+        check_moves(opt, before)
+        n = gdp.flatp.n_cast
+        assert torch.equal(gdp.flatp.shadow, gdp.flatp.flat[:n].bfloat16())
+        # and the vectors
+        assert bool((opt.flatp.flat[n:] != before[n:]).float().mean() > 0.9)
+    gdp.shutdown()
+
+
+def test_channels_last_weights_move_alike():
+    """A convolution's matrix in another order of its columns: the same
+    step, in that order."""
+    torch.manual_seed(9)
+    nets = [torch.nn.Sequential(torch.nn.Conv2d(24, 70, 3, bias=False),
+                                torch.nn.Conv2d(70, 130, 5, bias=False))
+            for _ in range(2)]
+    nets[1].load_state_dict(nets[0].state_dict())
+    nets[1].to(memory_format=torch.channels_last)
+    opts = [FusedMuon(FlatParams(net.to(dev()), flatten_grads=True), lr=0.1)
+            for net in nets]
+    start = [p.detach().clone() for p in nets[0].parameters()]
+    for p, q in zip(nets[0].parameters(), nets[1].parameters()):
+        assert p.stride() != q.stride() and torch.equal(p, q)
+        p.grad.normal_()
+        q.grad.copy_(p.grad)
+    # with a momentum of 0 before, u = (1 + mu) g, whose size does not count
+    grads = [p.grad.detach().clone() for p in nets[0].parameters()]
+    for opt in opts:
+        opt.step()
+    for p, q, s, g in zip(nets[0].parameters(), nets[1].parameters(), start,
+                          grads):
+        plain, ref = plain_error(g.flatten(1))
+        scale = 0.1 * max(1.0, ref.shape[0] / ref.shape[1]) ** 0.5
+        want = s.double() - scale * ref.view_as(s)
+        bound = scale * (4 * plain + input_roundings(g.flatten(1))) \
+            + 8 * 2.0 ** -24 * float(want.norm())
+        for t in (p, q):
+            assert float((t.detach().double() - want).norm()) <= bound
