@@ -24,17 +24,22 @@
 
 namespace {
 
+// N: values in 16 bytes; ZERO: the largest that rounds to 0, half of the
+// type's smallest
 template <typename T> struct Pack;
 template <> struct Pack<__bf16> {
   static constexpr int N = 8;
+  static constexpr float ZERO = 0x1p-134f;
   typedef __bf16 V __attribute__((ext_vector_type(8)));
 };
 template <> struct Pack<_Float16> {
   static constexpr int N = 8;
+  static constexpr float ZERO = 0x1p-25f;
   typedef _Float16 V __attribute__((ext_vector_type(8)));
 };
 template <> struct Pack<float> {
   static constexpr int N = 4;
+  static constexpr float ZERO = 0.f;
   typedef float V __attribute__((ext_vector_type(4)));
 };
 
@@ -115,7 +120,8 @@ __device__ __forceinline__ void put_w(void* w, bool w32, int64_t c, float f) {
 // that there is no gradient.
 template <typename T>
 __device__ __forceinline__ float rectify(float z) {
-  return z <= 0.f ? 0.f : (float)(T)z == 0.f ? -0.f : z;
+  const float f = z > 0.f ? -0.f : 0.f;
+  return !(z <= Pack<T>::ZERO) ? z : f;
 }
 __device__ __forceinline__ bool was_cut(float y) {
   return __float_as_uint(y) == 0;
@@ -215,8 +221,11 @@ __global__ __launch_bounds__(block_of(TPR)) void k_ln_fwd(
       for (int j = 0; j < N; ++j) {
         float z = ((float)now[i][j] - mean) * rstd * wv[i][j] + bv[i][j];
         if (res != nullptr) z += (float)now_res[i][j];
-        f[j] = relu ? rectify<T>(z) : z;
+        f[j] = z;
       }
+      if (relu)
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = rectify<T>(f[j]);
       store<T>(y + r * C, (t + i * TPR) * N, C, f);
     }
     if (mean_out != nullptr && t == 0) {
@@ -277,8 +286,11 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(
       for (int j = 0; j < N; ++j) {
         float z = (f[j] - mean) * rstd * wv[j] + bv[j];
         if (res != nullptr) z += a[j];
-        f[j] = relu ? rectify<T>(z) : z;
+        f[j] = z;
       }
+      if (relu)
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = rectify<T>(f[j]);
       store<T>(y + r * C, (int)c, C, f);
     }
     if (mean_out != nullptr && threadIdx.x == 0) {
