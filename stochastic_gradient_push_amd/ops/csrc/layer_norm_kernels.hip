@@ -14,9 +14,10 @@
 //
 // Bound by memory: each row is read once per pass and written once.  100352 x
 // 256 bf16 with residual and ReLU: forward 30 us (5.1 TB/s), backward 43 us
-// (6.0) and 5 us for the column sums; 4096 x 16384 fp16 62 us (4.3), 98 us
-// (4.1) and 14 us; 8191 x 1001 fp32 16 us, 23 us and 9 us.  Below about 5 MB
-// the launches count, 3 us each, and autograd's way to them, 50 us.
+// (6.0) and 5 us for the column sums; 4096 x 16384 fp16 59 us (4.6), 101 us
+// (4.0, with registers spilled) and 14 us; 8191 x 1001 fp32 16 us, 23 us and
+// 9 us.  Below about 5 MB the launches count, 3 us each, and autograd's way to
+// them, 50 us.
 
 #include <hip/hip_runtime.h>
 
@@ -555,7 +556,9 @@ __global__ __launch_bounds__(1024) void k_ln_bwd_sum(
 // ---------------------------------------------------------------- launch
 // The narrowest row group that holds a row in registers: short rows share
 // a wave, longer ones have a wave or a block.  Two vectors a thread at most:
-// with four, the backward pass has 200 registers and more, and spills.
+// with four, the backward pass has 200 registers and more.  With two it fits,
+// but for 16-bit rows over 8192: 1024 threads may have 128 registers each, and
+// 16 of those needed (23 with a ReLU) are spilled, 68 (80) bytes a thread.
 constexpr int MAX_VECTORS = 1024 * 2;
 
 #define LN_FOR_SHAPE(nv, CALL)                                     \

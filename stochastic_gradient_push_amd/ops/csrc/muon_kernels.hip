@@ -14,7 +14,8 @@
 // Two steps take 3 n^2 m + 5 n^3 operations like this instead of 6 n^2 m +
 // 2 n^3 (symmetric results count half).  A's error grows within the group, as
 // that of a recomputed A does not: groups are of two steps where the result
-// is fp32 itself, of three elsewhere.
+// is fp32 itself, of three where it is rounded to 16 bits, or is a step of
+// parameters whose own rounding is larger.
 //
 // All products run on the matrix cores, as row-by-row products C = P Q^T of
 // two operands whose rows lie along K: A = X X^T, A^2 = A A^T, and B X from
@@ -26,15 +27,17 @@
 // TFLOP/s of fp16 work, as a large fp16 library product does; the matrix
 // pipes are busy 67% of the time at the 1.6 GHz that the power limit leaves.
 // Around 1000: the 64 x 64 tiles' loads, 95 GB/s a CU (nothing but loads: 145
-// from L2, 90 to 120 from behind it).  Below 500: the 17 to 21 launches, 4 us
-// each.
+// from L2, 90 to 120 from behind it).  That is half of an n x n product's 11
+// us; the rest is its start, the sum over four waves and two passes of stores,
+// in each of 17 to 19 launches.  Below 500 the launches count, 4 us each.
 //
 // Precision.  A small singular value grows by the factor a in every step,
 // a^5 = 485 in all with the usual coefficients, and the rounding of X, A
 // and B grows with it.  Values are therefore held as two fp16 numbers,
 // v = hi + lo (22 bits), and a product is hi hi + hi lo + lo hi, three
-// matrix instructions with fp32 accumulation: errors are those of products
-// in fp32 or below (1000 x 2048: 1.0e-6 against 3.2e-6).  The last steps of
+// matrix instructions with fp32 accumulation: errors are about those of
+// products in fp32, mostly below (1000 x 2048 1.5e-6 against 3.4e-6, a step
+// over a small network 3.9e-8 against 3.8e-8).  The last steps of
 // a bf16 result, whose roundings can hardly grow any more, may keep hi alone:
 // only where the caller has asked for it, and the host says from which step
 // on.
@@ -1022,7 +1025,8 @@ __global__ __launch_bounds__(256) void k_ns_small(
 }
 
 // Workspace, in fp16 values: X and its transpose twice, A, B A, B and P
-// twice, each as two planes; x_total and a_total: the sizes of one plane.
+// twice, each as two planes; x_total and a_total: the sizes of one plane.  16
+// bytes a padded value of X and 20 a value of A: 533 MB for ResNet-50.
 struct Work {
   Planes x[2], xt[2], a, t, b, p[2];
 };
@@ -1119,7 +1123,9 @@ void ns_steps(Src src, const Work& w, int steps, int split_steps, int group,
 //   512 x 1024 148, 156   512 x 2048 175, 170   1000 x 2048 237, 235
 //   1024 x 1536 218, 223   2048 x 2560 772, 781   2048 x 4096 1022, 944
 //   4 of 512 x 1024 173, 169   4096 x 8192 6036, 5140
-// so from m = 3 n on, and from m = 2 n on where the difference is large.
+// so from m = 3 n on, and from m = 2 n on where the difference n^2 m - n^3 is
+// large: 4e8 lies between one 512 x 1024 (1.3e8) and four (5.4e8).  Around the
+// borders the two are within 5% of each other.
 int group_of(int most, double sum_nnm, double sum_nnn) {
   const double more = sum_nnm - sum_nnn;
   return more >= 2.0 * sum_nnn || (more >= sum_nnn && more >= 4e8) ? most : 1;
@@ -1136,11 +1142,12 @@ int64_t big_tiles(int64_t tiles) {
   return left <= 171 ? tiles - left : tiles;
 }
 
-// In a plan the sums differ, and a round of two tiles on each CU ends with its
-// longest: whole rounds only, and of the symmetric products, where they last
-// longest, none in one round (us a step: the 241 of ResNet-50 1015 and 793,
-// 394 of ResNet-101 1306 and 1147, 523 of ResNet-152 1545 and 1415; but 723
-// of three ResNet-50 2100 and 2196).
+// In a plan the sums differ, and a round of two tiles on each of 256 CUs ends
+// with its longest: whole rounds of 512 only.  Of the symmetric products, where
+// they last longest, none before a round and a quarter (us a step, with tiles
+// of 128 and without: the 241 of ResNet-50 1015 and 793, 394 of ResNet-101 1306
+// and 1147, 523 of ResNet-152 1545 and 1415; but 723 of three ResNet-50 2100
+// and 2196; between 523 and 723 nothing was measured).
 int64_t plan_big_tiles(int64_t tiles, bool sym) {
   return sym && tiles < 640 ? 0 : tiles - tiles % 512;
 }

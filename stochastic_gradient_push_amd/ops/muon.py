@@ -6,6 +6,9 @@ flat parameter buffer (``csrc/muon_kernels.hip``).
     X = G / (|G|_F + eps);   steps times:  X = (a I + b A + c A^2) X,
                                            A = X X^T
 
+(the Newton-Schulz iteration for a polar factor with a quintic instead of the
+classic cubic).
+
 ``muon_step_`` is one optimiser step of every matrix in a flat buffer (the
 layout of :class:`~stochastic_gradient_push_amd.ops.flat.FlatParams`), all
 shapes together in one launch per product; what lies between the matrices
@@ -18,7 +21,9 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-#: slope at zero as large as convergence into [0.68, 1.21] allows
+#: slope at zero as large as convergence into [0.68, 1.21] allows; from the
+#: publication of the method: K. Jordan et al., "Muon: An optimizer for hidden
+#: layers in neural networks", 2024, like the update's scale in a step
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
@@ -120,6 +125,10 @@ def newton_schulz(
     one with a NaN or an infinity becomes NaN as a whole.  Not differentiable:
     a ``g`` that requires a gradient is refused, on the device a dual one and
     a call under ``torch.jit.trace`` or ``make_fx`` too.
+
+    Workspace on the device: 16 bytes a value and 20 bytes a value of a square
+    of the smaller side, both sides padded to multiples of 64, for the whole
+    batch; none up to 64 x 192 (or 192 x 64).
     """
     if g.dim() < 2:
         raise ValueError("newton_schulz: g must be a matrix or a batch of "
@@ -214,6 +223,8 @@ def muon_step_(
     ``shadow``, where given, receives the new parameters in bf16.  ``lr`` is
     a float, or one value on the device that a captured step reads anew.
     Not recorded by autograd; the device refuses dual tensors and tracing.
+    Its workspace is that of ``newton_schulz`` for all matrices at once (16
+    bytes a value and 20 a value of the smaller sides' squares, padded).
     """
     coefficients = _check_numbers("muon_step_", steps, coefficients, eps)
     growth = _growth(coefficients, steps)
